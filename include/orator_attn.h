@@ -97,6 +97,20 @@ int orator_rope_half(float* x, const int* positions, int n_tokens, int n_heads, 
  * Same tie rule: ties keep the candidate of the lower scan slot. */
 int orator_argmax_banned(const float* logits, int n, int ban0, int ban1, int* out_idx,
                          void* stream);
+/* No counterpart in the reference: the log probability of a given token, the entropy and the best
+ * alternatives of each row of logits [rows][vocab] (fp32, row r at r * row_stride elements), as the
+ * confidence of a transcription takes them.  With lse = log sum_i exp(x_i):
+ *   logprob[r]      x[tokens[r]] - lse (NaN for a token outside [0, vocab))
+ *   entropy[r]      lse - sum_i p_i x_i, in nats; entries of -infinity (banned ids) count nothing
+ *   top_ids[r][k]   the ids of the top_k largest logits, largest first, ties to the lowest id
+ *   top_logprobs    their x - lse
+ * Any of the outputs may be NULL (top_ids and top_logprobs together; tokens with logprob).
+ * 0 <= top_k <= 32, top_k <= vocab.  A row of -infinity only has log probabilities -infinity and
+ * entropy 0; a row with a NaN or +infinity has NaN for both (ids: NaN ranks below every number,
+ * -infinity included). */
+int orator_token_logprobs(const float* logits, long row_stride, const int* tokens, int rows,
+                          int vocab, int top_k, float* logprob, float* entropy, int* top_ids,
+                          float* top_logprobs, void* stream);
 /* asr_ops::GqaAttention (include/model/asr_ops.cuh:50-56; src/model/asr_ops.cu:130-195,252-295).
  * fp32 q [T,Hq,Dh], k/v [T,Hkv,Dh]; row i attends keys [0,i] (causal) or [0,T).  Default
  * stream.  As the reference: any power-of-two Dh <= 1024 and any Hq that is a multiple of Hkv
@@ -220,6 +234,84 @@ int orator_gqa_decode_append_paged(const float* q, const float* k_new, const flo
                                    int max_pages, int page_size, int n_pages, const int* d_pos,
                                    float* out, int B, int Hq, int Hkv, int Dh, float scale,
                                    void* stream);
+
+/* ------------------------------------------------------------ KV cache in 8 bits ---- */
+/* No counterpart in the reference: a KV cache of one byte per value and one fp32 scale per
+ * position and kv head, 0.52 of the bf16 cache's bytes at Dh 128.
+ *
+ * A row of Dh values x is held as scale = max|x| * (1 / 127), both in fp32, and codes = the
+ * integers nearest to x / scale (ties to even, in [-127, 127]); it reads back as code * scale, each
+ * value within scale / 2 of x.  A row whose scale would be subnormal (max|x| < 127 * 2^-126) is held as zeros,
+ * a row with an infinity or a NaN as scale NaN (it reads back as NaN, and so does an attention
+ * that attends it).
+ *
+ * Layout, in pages of page_size positions (a power of two >= 16):
+ *   K codes  kq [n_pages][Hkv][page_size][Dh]            int8
+ *   V codes  vq [n_pages][Hkv][page_size / 16][Dh][16]   int8: blocks of 16 positions, dims outside
+ *   scales   ks, vs [n_pages][Hkv][page_size]            fp32
+ * page_table[b * max_pages + i] names the page of stream b's positions [i * page_size,
+ * (i + 1) * page_size).  A contiguous cache is one page of `capacity` positions (capacity a
+ * multiple of 16).  kq, vq, ks and vs are 16-byte aligned.  Dh: a multiple of 16, at most 256 (64
+ * and 128 run on the kernels built for them, others on generic ones).  Pages named by a negative
+ * entry or one >= n_pages are unmapped: they are neither written nor read. */
+
+/* The rows k, v [Tq][Hkv][Dh] (fp32, row t at t * kv_stride elements, heads contiguous) go to
+ * positions *d_pos0 + t.  Rows outside [0, capacity) are not written. */
+int orator_kv_write_q8(const float* k, const float* v, long kv_stride, int8_t* kq, float* ks,
+                       int8_t* vq, float* vs, int Tq, int Hkv, int Dh, const int* d_pos0,
+                       int capacity, void* stream);
+/* Paged form: stream b's Tq rows (row t at (b * Tq + t) * kv_stride) go to positions d_pos0[b] + t
+ * through page-table row b.  Rows outside the table or of unmapped pages are not written; two
+ * streams must not write the same page. */
+int orator_kv_write_q8_paged(const float* k, const float* v, long kv_stride, int8_t* kq, float* ks,
+                             int8_t* vq, float* vs, const int* page_table, int max_pages,
+                             int page_size, int n_pages, int B, int Tq, int Hkv, int Dh,
+                             const int* d_pos0, void* stream);
+/* The values held for positions *d_pos0 + t, t < Tq, into k, v [Tq][Hkv][Dh]: bf16 (out_bf16 = 1,
+ * rows that the bf16 prefill reads) or fp32 (out_bf16 = 0): fl32(code * scale), rounded to bf16.
+ * Rows outside [0, capacity) are left as they were. */
+int orator_kv_read_q8(const int8_t* kq, const float* ks, const int8_t* vq, const float* vs,
+                      void* k, void* v, int out_bf16, int Tq, int Hkv, int Dh, const int* d_pos0,
+                      int capacity, void* stream);
+/* Paged form, into k, v [B][Tq][Hkv][Dh]; rows outside the table or of unmapped pages are left as
+ * they were. */
+int orator_kv_read_q8_paged(const int8_t* kq, const float* ks, const int8_t* vq, const float* vs,
+                            const int* page_table, int max_pages, int page_size, int n_pages,
+                            void* k, void* v, int out_bf16, int B, int Tq, int Hkv, int Dh,
+                            const int* d_pos0, void* stream);
+/* orator_gqa_decode over the 8-bit cache: q [Hq, Dh] fp32 attends the *d_pos + 1 keys, clamped to
+ * the capacity (*d_pos < 0: no key, zeros).  Any Hq that is a multiple of Hkv.  The products are
+ * exact in the codes; q and the softmax weights keep fp32 accuracy. */
+int orator_gqa_decode_q8(const float* q, const int8_t* kq, const float* ks, const int8_t* vq,
+                         const float* vs, float* out, int Hq, int Hkv, int Dh, const int* d_pos,
+                         int capacity, float scale, void* stream);
+/* Batched paged form: stream b's q [Hq, Dh] attends d_pos[b] + 1 keys through page-table row b;
+ * keys of unmapped pages are not attended.  q/out [B, Hq, Dh]. */
+int orator_gqa_decode_q8_paged(const float* q, const int8_t* kq, const float* ks, const int8_t* vq,
+                               const float* vs, const int* page_table, int max_pages,
+                               int page_size, int n_pages, const int* d_pos, float* out, int B,
+                               int Hq, int Hkv, int Dh, float scale, void* stream);
+
+/* --------------------------------------------------------- decode behind one prefix ---- */
+/* No counterpart in the reference: orator_gqa_decode_paged for a batch whose first shared_len
+ * positions are the same rows for every stream (one prompt for all sessions).  Those keys are read
+ * once for the whole batch, through page-table row 0; the keys from shared_len on through each
+ * stream's own row (the entries of rows b > 0 for pages wholly inside the prefix are not read).
+ * Stream b attends d_pos[b] + 1 keys: only the first of the prefix's where that is fewer than
+ * shared_len, none (zeros) where d_pos[b] < 0.  Keys of unmapped pages (negative or >= n_pages)
+ * are not attended.  shared_len in [0, max_pages * page_size], page_size a power of two >= 16, any
+ * B, any Hq that is a multiple of Hkv; Dh a multiple of 16, at most 256 (64 and 128 run on the
+ * matrix cores).  Results as orator_gqa_decode_paged's, to fp32 rounding. */
+int orator_gqa_decode_shared_paged(const float* q, const uint16_t* kpool, const uint16_t* vpool,
+                                   const int* page_table, int max_pages, int page_size,
+                                   int n_pages, const int* d_pos, int shared_len, float* out,
+                                   int B, int Hq, int Hkv, int Dh, float scale, void* stream);
+/* The same over the 8-bit cache. */
+int orator_gqa_decode_shared_q8_paged(const float* q, const int8_t* kq, const float* ks,
+                                      const int8_t* vq, const float* vs, const int* page_table,
+                                      int max_pages, int page_size, int n_pages, const int* d_pos,
+                                      int shared_len, float* out, int B, int Hq, int Hkv, int Dh,
+                                      float scale, void* stream);
 
 /* WindowAttnKernel (src/model/asr_audio_tower.cu:204-258, launch :573-575): the audio tower's
  * self-attention, q/k/v fp32 [N, H, Dh] (Dh in [1, 1024]; 64 and 128 on the fast kernels);

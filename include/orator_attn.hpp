@@ -66,6 +66,13 @@ inline void ArgmaxBanned(const float* logits, int n, int ban0, int ban1, int* ou
   gpu::Check(orator_argmax_banned(logits, n, ban0, ban1, out_idx, stream));
 }
 
+inline void TokenLogprobs(const float* logits, long row_stride, const int* tokens, int rows,
+                          int vocab, int top_k, float* logprob, float* entropy, int* top_ids,
+                          float* top_logprobs, hipStream_t stream = 0) {
+  gpu::Check(orator_token_logprobs(logits, row_stride, tokens, rows, vocab, top_k, logprob,
+                                   entropy, top_ids, top_logprobs, stream));
+}
+
 }  // namespace asr_ops
 
 namespace asr_gemm {  // include/model/asr_gemm.h:23-41
@@ -124,6 +131,26 @@ inline void QkNormRopeKvWrite(float* q, float* k, const float* v, long q_stride,
   gpu::Check(orator_qk_norm_rope_kv_write(q, k, v, q_stride, kv_stride, q_norm, k_norm, eps,
                                           positions, theta, n_tokens, n_tokens, Hq, Hkv, Dh, kc,
                                           vc, nullptr, 0, 0, capacity, stream));
+}
+
+// The KV cache in 8 bits: one page of `capacity` positions (a multiple of 16).
+inline void WriteKvCacheQ8(const float* k, const float* v, long kv_stride, int8_t* kq, float* ks,
+                           int8_t* vq, float* vs, int Tq, int Hkv, int Dh, const int* d_pos0,
+                           int capacity, hipStream_t stream = 0) {
+  gpu::Check(orator_kv_write_q8(k, v, kv_stride, kq, ks, vq, vs, Tq, Hkv, Dh, d_pos0, capacity,
+                                stream));
+}
+inline void ReadKvCacheQ8(const int8_t* kq, const float* ks, const int8_t* vq, const float* vs,
+                          void* k, void* v, bool out_bf16, int Tq, int Hkv, int Dh,
+                          const int* d_pos0, int capacity, hipStream_t stream = 0) {
+  gpu::Check(orator_kv_read_q8(kq, ks, vq, vs, k, v, out_bf16 ? 1 : 0, Tq, Hkv, Dh, d_pos0,
+                               capacity, stream));
+}
+inline void GqaDecodeAttnQ8(const float* q, const int8_t* kq, const float* ks, const int8_t* vq,
+                            const float* vs, float* out, int Hq, int Hkv, int Dh, const int* d_pos,
+                            int capacity, float scale, hipStream_t stream = 0) {
+  gpu::Check(orator_gqa_decode_q8(q, kq, ks, vq, vs, out, Hq, Hkv, Dh, d_pos, capacity, scale,
+                                  stream));
 }
 
 }  // namespace decoder_attn

@@ -114,6 +114,7 @@ SIGNATURES: dict[str, list] = {
     "orator_swiglu": [_p, _p, _p, _i, _p],
     "orator_rope_half": [_p, _p, _i, _i, _i, _f, _p],
     "orator_argmax_banned": [_p, _i, _i, _i, _p, _p],
+    "orator_token_logprobs": [_p, _l, _p, _i, _i, _i, _p, _p, _p, _p, _p],
     "orator_gqa_attention": [_p, _p, _p, _p, _i, _i, _i, _i, _f, _i],
     "orator_f32_to_bf16": [_p, _p, _l, _p],
     "orator_bf16_to_f32": [_p, _p, _l, _p],
@@ -128,6 +129,20 @@ SIGNATURES: dict[str, list] = {
                                         _f, _p, _i, _p],
     "orator_gqa_decode_append_qknorm_paged": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _i, _i,
                                               _i, _i, _f, _p, _p, _f, _p, _i, _p],
+    # KV cache in 8 bits, and decode behind a shared prefix
+    "orator_kv_write_q8": [_p, _p, _l, _p, _p, _p, _p, _i, _i, _i, _p, _i, _p],
+    "orator_kv_write_q8_paged": [_p, _p, _l, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p,
+                                 _p],
+    "orator_kv_read_q8": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _i, _p],
+    "orator_kv_read_q8_paged": [_p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _i, _i, _i, _i, _i, _p,
+                                _p],
+    "orator_gqa_decode_q8": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _p, _i, _f, _p],
+    "orator_gqa_decode_q8_paged": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _i, _i, _i, _i, _f,
+                                   _p],
+    "orator_gqa_decode_shared_paged": [_p, _p, _p, _p, _i, _i, _i, _p, _i, _p, _i, _i, _i, _i, _f,
+                                       _p],
+    "orator_gqa_decode_shared_q8_paged": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _p, _i, _p, _i, _i,
+                                          _i, _i, _f, _p],
     "orator_rope_table": [_p, _i, _f, _p],
     "orator_conformer_create": [_i, _i, _i, _i, C.POINTER(ConformerWeights), C.POINTER(_p)],
     "orator_conformer_destroy": [_p],

@@ -47,6 +47,14 @@ def ArgmaxBanned(logits, n: int, ban0: int, ban1: int, out_idx, stream=None) -> 
     call("orator_argmax_banned", ptr(logits), n, ban0, ban1, ptr(out_idx), _sh(stream))
 
 
+def TokenLogprobs(logits, row_stride: int, tokens, rows: int, vocab: int, top_k: int, logprob,
+                  entropy, top_ids, top_logprobs, stream=None) -> None:
+    """Per row of logits [rows, vocab]: the log probability of tokens[r], the entropy, and the
+    top_k ids (ties to the lowest) with their log probabilities; outputs may be None."""
+    call("orator_token_logprobs", ptr(logits), row_stride, ptr(tokens), rows, vocab, top_k,
+         ptr(logprob), ptr(entropy), ptr(top_ids), ptr(top_logprobs), _sh(stream))
+
+
 def F32ToBf16(inp, out, n: int, stream=None) -> None:
     """include/model/asr_gemm.h:24."""
     call("orator_f32_to_bf16", ptr(inp), ptr(out), n, _sh(stream))

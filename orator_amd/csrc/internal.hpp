@@ -31,8 +31,15 @@ constexpr int kWsGemm = 1;
 constexpr int kWsArrive = 3;  // arrival counters of the decode's in-launch split merge
 constexpr int kWsPrefill = 4;        // partials of the long-prompt prefill's cut blocks
 constexpr int kWsPrefillArrive = 5;  // its arrival counters
+constexpr int kWsKeys = 6;       // partials of the 8-bit cache's and the shared prefix's attention
+constexpr int kWsLogprobs = 7;   // partials of the token log probabilities
 // *fresh (optional): the block was allocated by this call, its contents undefined.
 void* workspace(hipStream_t stream, size_t bytes, int slot = 0, bool* fresh = nullptr);
+// workspace() for the operators whose captured calls need no reserve call before the capture: while
+// `stream` is being captured the block belongs to that capture alone (allocated within it, kept
+// until workspace_release(stream)), so graphs captured on one stream share no scratch and may be
+// replayed at the same time on several, or beside eager calls.
+void* workspace_graph(hipStream_t stream, size_t bytes, int slot, bool* fresh = nullptr);
 
 // Whether workspace() serves `bytes` without allocating while `stream` is being captured (where HIP
 // refuses it): always when it is not.
@@ -242,5 +249,40 @@ int launch_sgemm_group3(const float* in, const float* const W[3], const float* c
 // an fp16 consumer would round from launch_sgemm's fp32 output.
 int launch_sgemm_f16_out(const float* in, const float* W, void* out, int M, int K, int N,
                          hipStream_t stream);
+
+// Decode attention over paged keys for the entries that take the 8-bit cache or a shared prefix:
+// stream b attends keys j < min(pos[b] + 1, capacity), those below shared_len through page-table
+// row 0.  Keys of unmapped pages are not attended.
+struct KeysProblem {
+  const float* q;            // [B][Hq][Dh]
+  bool bf16;                 // kpool and vpool are the cache; otherwise kq, ks, vq and vs
+  const uint16_t* kpool;     // bf16 pool [page][page_size][Hkv][Dh]
+  const uint16_t* vpool;
+  const int8_t* kq;
+  const float* ks;
+  const int8_t* vq;
+  const float* vs;
+  const int* page_table;     // null: contiguous (8-bit cache only)
+  int max_pages, page_size, n_pages;
+  int capacity;              // contiguous
+  const int* pos;
+  int shared_len;
+  float* out;
+  int B, Hq, Hkv, Dh;
+  float scale;
+};
+// Any Dh that is a multiple of 16 up to 256, any group (decode_keys_generic.hip).
+struct Q8Map;
+int launch_keys_generic(const KeysProblem& p, const Q8Map& map, hipStream_t stream);
+
+// Runs an entry point's body; an exception (of the host's allocations) becomes a status.
+template <typename F>
+int guarded(F&& body) {
+  try {
+    return body();
+  } catch (...) {
+    return ORATOR_ERR_CAPACITY;
+  }
+}
 
 }  // namespace orator_hip

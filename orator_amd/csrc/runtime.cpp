@@ -18,7 +18,23 @@ namespace orator_hip {
 namespace {
 thread_local std::string g_last_error;
 
-int ws_alloc(void** p, size_t bytes) { return hipMalloc(p, bytes) == hipSuccess ? 0 : 1; }
+// Set while a block of a captured graph is allocated (workspace_graph).
+thread_local bool g_ws_relaxed = false;
+
+int ws_alloc(void** p, size_t bytes) {
+  if (!g_ws_relaxed) return hipMalloc(p, bytes) == hipSuccess ? 0 : 1;
+  // An allocation is no part of the graph being captured: the thread's capture mode is relaxed
+  // around it, or hipMalloc would refuse and end the capture.
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) {
+    (void)hipGetLastError();
+    return 1;
+  }
+  const hipError_t e = hipMalloc(p, bytes);
+  (void)hipThreadExchangeStreamCaptureMode(&mode);
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e == hipSuccess ? 0 : 1;
+}
 void ws_free(void* p) { (void)hipFree(p); }
 int ws_sync(const void* stream) {
   return hipStreamSynchronize(static_cast<hipStream_t>(const_cast<void*>(stream))) == hipSuccess
@@ -114,6 +130,29 @@ void* workspace(hipStream_t stream, size_t bytes, int slot, bool* fresh) {
   g_ws_guard.armed = true;
   void* p = ws_pool().get(WsKey{dev, stream, std::this_thread::get_id(), slot}, bytes,
                           ws_capturing(stream), &err, fresh);
+  if (!p) (void)fail(ORATOR_ERR_HIP, err);
+  return p;
+}
+
+void* workspace_graph(hipStream_t stream, size_t bytes, int slot, bool* fresh) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (check_hip(hipStreamGetCaptureInfo(stream, &st, &id), "hipStreamGetCaptureInfo") != ORATOR_OK)
+    return nullptr;
+  if (st == hipStreamCaptureStatusNone) return workspace(stream, bytes, slot, fresh);
+  if (st != hipStreamCaptureStatusActive) {
+    (void)fail(ORATOR_ERR_HIP, "workspace: the stream's capture is no longer valid");
+    return nullptr;
+  }
+  int dev = 0;
+  if (check_hip(hipGetDevice(&dev), "hipGetDevice") != ORATOR_OK) return nullptr;
+  std::string err;
+  g_ws_guard.armed = true;
+  g_ws_relaxed = true;
+  // capture ids start at 1 and are not used twice; 0 would be the stream's eager block
+  void* p = ws_pool().get(WsKey{dev, stream, std::this_thread::get_id(), slot, id + 1}, bytes, true,
+                          &err, fresh);
+  g_ws_relaxed = false;
   if (!p) (void)fail(ORATOR_ERR_HIP, err);
   return p;
 }

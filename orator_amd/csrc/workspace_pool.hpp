@@ -37,8 +37,12 @@ struct WsKey {
   const void* stream;
   std::thread::id tid;
   int slot = 0;  // independent blocks for buffers that are live at the same time
+  // The capture a block belongs to (0: none), for the operators whose captured calls keep a block
+  // per graph: graphs that are replayed at the same time then share no scratch.
+  unsigned long long capture = 0;
   bool operator<(const WsKey& o) const {
-    return std::tie(dev, stream, tid, slot) < std::tie(o.dev, o.stream, o.tid, o.slot);
+    return std::tie(dev, stream, tid, slot, capture) <
+           std::tie(o.dev, o.stream, o.tid, o.slot, o.capture);
   }
 };
 

@@ -132,3 +132,71 @@ def GqaDecodeAttnAppendQkNormPaged(q, k_new, v_new, kpool, vpool, page_table, ma
     call("orator_gqa_decode_append_qknorm_paged", ptr(q), ptr(k_new), ptr(v_new), ptr(kpool),
          ptr(vpool), ptr(page_table), max_pages, page_size, n_pages, ptr(d_pos), ptr(out), B, Hq,
          Hkv, Dh, scale, ptr(q_norm), ptr(k_norm), eps, ptr(rope), rope_rows, _sh(stream))
+
+
+# ---- KV cache in 8 bits: codes kq / vq, fp32 scales ks / vs per position and kv head ----
+def WriteKvCacheQ8(k, v, kv_stride: int, kq, ks, vq, vs, Tq: int, Hkv: int, Dh: int, d_pos0,
+                   capacity: int, stream=None) -> None:
+    """Quantises fp32 rows k/v (row t at t * kv_stride) into positions *d_pos0 + t."""
+    call("orator_kv_write_q8", ptr(k), ptr(v), kv_stride, ptr(kq), ptr(ks), ptr(vq), ptr(vs), Tq,
+         Hkv, Dh, ptr(d_pos0), capacity, _sh(stream))
+
+
+def WriteKvCacheQ8Paged(k, v, kv_stride: int, kq, ks, vq, vs, page_table, max_pages: int,
+                        page_size: int, n_pages: int, B: int, Tq: int, Hkv: int, Dh: int, d_pos0,
+                        stream=None) -> None:
+    """Stream b's Tq rows go to positions d_pos0[b] + t through page-table row b."""
+    call("orator_kv_write_q8_paged", ptr(k), ptr(v), kv_stride, ptr(kq), ptr(ks), ptr(vq),
+         ptr(vs), ptr(page_table), max_pages, page_size, n_pages, B, Tq, Hkv, Dh, ptr(d_pos0),
+         _sh(stream))
+
+
+def ReadKvCacheQ8(kq, ks, vq, vs, k, v, out_bf16: bool, Tq: int, Hkv: int, Dh: int, d_pos0,
+                  capacity: int, stream=None) -> None:
+    """The values held for positions *d_pos0 + t into k/v [Tq, Hkv, Dh], bf16 or fp32."""
+    call("orator_kv_read_q8", ptr(kq), ptr(ks), ptr(vq), ptr(vs), ptr(k), ptr(v),
+         int(bool(out_bf16)), Tq, Hkv, Dh, ptr(d_pos0), capacity, _sh(stream))
+
+
+def ReadKvCacheQ8Paged(kq, ks, vq, vs, page_table, max_pages: int, page_size: int, n_pages: int, k,
+                       v, out_bf16: bool, B: int, Tq: int, Hkv: int, Dh: int, d_pos0,
+                       stream=None) -> None:
+    """ReadKvCacheQ8 of B streams through their page-table rows, into k/v [B, Tq, Hkv, Dh]."""
+    call("orator_kv_read_q8_paged", ptr(kq), ptr(ks), ptr(vq), ptr(vs), ptr(page_table),
+         max_pages, page_size, n_pages, ptr(k), ptr(v), int(bool(out_bf16)), B, Tq, Hkv, Dh,
+         ptr(d_pos0), _sh(stream))
+
+
+def GqaDecodeAttnQ8(q, kq, ks, vq, vs, out, Hq: int, Hkv: int, Dh: int, d_pos, capacity: int,
+                    scale: float, stream=None) -> None:
+    """GqaDecodeAttn over the 8-bit cache."""
+    call("orator_gqa_decode_q8", ptr(q), ptr(kq), ptr(ks), ptr(vq), ptr(vs), ptr(out), Hq, Hkv,
+         Dh, ptr(d_pos), capacity, scale, _sh(stream))
+
+
+def GqaDecodeAttnQ8Paged(q, kq, ks, vq, vs, page_table, max_pages: int, page_size: int,
+                         n_pages: int, d_pos, out, B: int, Hq: int, Hkv: int, Dh: int,
+                         scale: float, stream=None) -> None:
+    """GqaDecodeAttnPaged over the 8-bit cache."""
+    call("orator_gqa_decode_q8_paged", ptr(q), ptr(kq), ptr(ks), ptr(vq), ptr(vs),
+         ptr(page_table), max_pages, page_size, n_pages, ptr(d_pos), ptr(out), B, Hq, Hkv, Dh,
+         scale, _sh(stream))
+
+
+def GqaDecodeAttnSharedPaged(q, kpool, vpool, page_table, max_pages: int, page_size: int,
+                             n_pages: int, d_pos, shared_len: int, out, B: int, Hq: int, Hkv: int,
+                             Dh: int, scale: float, stream=None) -> None:
+    """GqaDecodeAttnPaged for streams whose first shared_len positions are the same rows (those
+    of page-table row 0), read once for the batch."""
+    call("orator_gqa_decode_shared_paged", ptr(q), ptr(kpool), ptr(vpool), ptr(page_table),
+         max_pages, page_size, n_pages, ptr(d_pos), shared_len, ptr(out), B, Hq, Hkv, Dh, scale,
+         _sh(stream))
+
+
+def GqaDecodeAttnSharedQ8Paged(q, kq, ks, vq, vs, page_table, max_pages: int, page_size: int,
+                               n_pages: int, d_pos, shared_len: int, out, B: int, Hq: int,
+                               Hkv: int, Dh: int, scale: float, stream=None) -> None:
+    """GqaDecodeAttnSharedPaged over the 8-bit cache."""
+    call("orator_gqa_decode_shared_q8_paged", ptr(q), ptr(kq), ptr(ks), ptr(vq), ptr(vs),
+         ptr(page_table), max_pages, page_size, n_pages, ptr(d_pos), shared_len, ptr(out), B, Hq,
+         Hkv, Dh, scale, _sh(stream))
