@@ -1231,11 +1231,11 @@ size_t decode_workspace_bytes(int B, int Hq, int Dh, int capacity) {
   return static_cast<size_t>(B) * Hq * max_splits * (Dh + 2) * sizeof(float);
 }
 
-int zeroed_counters(hipStream_t stream, int slot, unsigned** out) {
+int zeroed_counters(hipStream_t stream, int slot, unsigned** out, bool per_graph) {
   bool fresh = false;
-  *out = static_cast<unsigned*>(
-      workspace(stream, static_cast<size_t>(kArriveCounters) * kCounterStride * sizeof(unsigned),
-                slot, &fresh));
+  const size_t bytes = static_cast<size_t>(kArriveCounters) * kCounterStride * sizeof(unsigned);
+  *out = static_cast<unsigned*>(per_graph ? workspace_graph(stream, bytes, slot, &fresh)
+                                          : workspace(stream, bytes, slot, &fresh));
   if (!*out) return ORATOR_ERR_HIP;
   if (fresh) {
     hipLaunchKernelGGL(zero_u32_kernel, dim3(kArriveCounters * kCounterStride / 256), dim3(256), 0,

@@ -32,6 +32,7 @@ constexpr int kWsArrive = 3;  // arrival counters of the decode's in-launch spli
 constexpr int kWsPrefill = 4;        // partials of the long-prompt prefill's cut blocks
 constexpr int kWsPrefillArrive = 5;  // its arrival counters
 constexpr int kWsKeys = 6;       // partials of the 8-bit cache's and the shared prefix's attention
+constexpr int kWsKeysArrive = 8;  // their arrival counters
 constexpr int kWsLogprobs = 7;   // partials of the token log probabilities
 // *fresh (optional): the block was allocated by this call, its contents undefined.
 void* workspace(hipStream_t stream, size_t bytes, int slot = 0, bool* fresh = nullptr);
@@ -128,8 +129,8 @@ constexpr int kArriveCounters = 4096;
 constexpr int kCounterStride = 32;
 // A block of kArriveCounters counters (kCounterStride apart) in workspace slot `slot` of the
 // stream, zeroed by a fill kernel when the block is allocated; the kernels using it return
-// every counter to zero.
-int zeroed_counters(hipStream_t stream, int slot, unsigned** out);
+// every counter to zero.  per_graph: a captured call's block is its graph's own (workspace_graph).
+int zeroed_counters(hipStream_t stream, int slot, unsigned** out, bool per_graph = false);
 // Long-prompt bf16 prefill over a contiguous cache, one wave per SIMD with stream-K balance
 // (prefill_sk.hip); Dh 128, Hq / Hkv in {1, 2, 4}, Hkv * ceil(Tq / (128 / G)) <= kArriveCounters.
 int launch_prefill_sk(const float* q, const uint16_t* q_bf16, const uint16_t* kc,
@@ -274,6 +275,8 @@ struct KeysProblem {
 // Any Dh that is a multiple of 16 up to 256, any group (decode_keys_generic.hip).
 struct Q8Map;
 int launch_keys_generic(const KeysProblem& p, const Q8Map& map, hipStream_t stream);
+// Dh 64 and 128 over the 8-bit cache, no shared prefix (decode_q8.hip).
+int launch_decode_q8(const KeysProblem& p, const Q8Map& map, hipStream_t stream);
 
 // Runs an entry point's body; an exception (of the host's allocations) becomes a status.
 template <typename F>
