@@ -167,9 +167,9 @@ int decode_keys(const char* what, const KeysProblem& p, bool paged, hipStream_t 
   if (p.shared_len < 0) return fail(ORATOR_ERR_INVALID, who + ": shared_len must be >= 0");
   if (p.shared_len > map.capacity)
     return fail(ORATOR_ERR_CAPACITY, who + ": shared_len exceeds max_pages * page_size");
-  if (!p.bf16 && p.shared_len == 0 && (p.Dh == 64 || p.Dh == 128))
-    return launch_decode_q8(p, map, stream);
-  return launch_keys_generic(p, map, stream);
+  if (p.Dh != 64 && p.Dh != 128) return launch_keys_generic(p, map, stream);
+  if (!p.bf16 && p.shared_len == 0) return launch_decode_q8(p, map, stream);
+  return launch_shared_prefix(p, map, stream);
 }
 
 KeysProblem keys_problem(const float* q, const int* d_pos, float* out, int B, int Hq, int Hkv,

@@ -277,6 +277,8 @@ struct Q8Map;
 int launch_keys_generic(const KeysProblem& p, const Q8Map& map, hipStream_t stream);
 // Dh 64 and 128 over the 8-bit cache, no shared prefix (decode_q8.hip).
 int launch_decode_q8(const KeysProblem& p, const Q8Map& map, hipStream_t stream);
+// Dh 64 and 128 over a paged cache of either kind (shared_prefix.hip).
+int launch_shared_prefix(const KeysProblem& p, const Q8Map& map, hipStream_t stream);
 
 // Runs an entry point's body; an exception (of the host's allocations) becomes a status.
 template <typename F>

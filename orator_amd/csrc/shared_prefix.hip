@@ -1,0 +1,468 @@
+// Decode attention of a batch whose streams share a prefix, over the bf16 pool or the 8-bit cache:
+// the prefix's keys are read once for all streams, gfx950.
+//
+// For one kv head, the B G query rows of the batch against the prefix are a matrix product, and so
+// are a stream's G rows against its own keys (G of 32 columns used: its time is its memory's).
+// One kernel does both; a workgroup has one unit of work, 32 query columns and a range of keys:
+//  * prefix units: columns are rows (stream, head) b G + g of the batch, keys [0, P) through
+//    page-table row 0;
+//  * own units: columns are the G heads of one stream, keys [P, S_b) through its own row.  A stream
+//    with fewer keys than the prefix has none there and is no column of a prefix unit: its unit
+//    takes keys [0, S_b) of row 0.  So a unit's columns all attend the same keys, and a value that
+//    is not finite reaches no stream that does not attend it (0 * inf in a product is NaN).
+//
+// Per 32-key tile of a wave, S^T = K Q^T and O^T += V^T W^T on mfma_f32_32x32x16_bf16:
+//  * q and the weights w enter as three bf16 terms (the top 8, middle 8 and last 8 bits of the
+//    fp32 significand, split by truncation: exact), K and V as they are (bf16, or int8 codes,
+//    which bf16 holds exactly): fp32 accuracy for 3 MFMAs per product.
+//  * a lane has one query column, and scores of 16 consecutive keys: tile row 8 a + 4 h + i is key
+//    16 h + 4 a + i, so lane half h holds block h of the tile and its registers are the B operand
+//    of the second product as they are.
+//  * V^T: bf16 rows through LDS and the transposing read; 8-bit codes lie transposed in memory, a
+//    lane's 16 bytes are its operand.
+//  * softmax with a reference that follows the running maximum once it is 8 (log2) behind.
+// The waves of a workgroup take the range's tiles in turn and are joined in LDS; the units'
+// partials of a (stream, head) by a second kernel.
+#include <algorithm>
+#include <string>
+
+#include "kv_q8.hpp"
+#include "mfma_tile.hpp"
+
+namespace orator_hip {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kTile = 32;     // keys per wave tile
+constexpr int kCols = 32;     // query columns of a unit
+constexpr float kSlack = 8.0f;
+
+struct SharedArgs {
+  KeysProblem p;
+  Q8Map map;
+  float scale_log2e;
+  int G;
+  int col_blocks;   // blocks of 32 rows of the batch
+  int n_pre;        // prefix units per (kv head, column block)
+  int pre_tiles;    // tiles per prefix unit
+  int n_own;        // own units per (stream, kv head, chunk of 32 heads)
+  int own_chunks;
+  int slots;        // n_pre + n_own: partials per (stream, head)
+  float* part_o;    // [B * Hq][slots][Dh]
+  float* part_ml;   // [B * Hq][slots][2]
+};
+
+__device__ __forceinline__ int stream_len(const SharedArgs& a, int b) {
+  const int pos = a.p.pos[b];
+  return pos < 0 ? 0 : min(pos, a.map.capacity - 1) + 1;
+}
+
+// Two fp32 to one dword of their upper halves (the bf16 that truncation gives).
+__device__ __forceinline__ uint32_t upper2(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+__device__ __forceinline__ float drop_upper(float x) {
+  return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+}
+
+// 8 fp32 as three bf16 terms; exact but for an infinity (NaN).
+__device__ __forceinline__ void split3(const float (&x)[8], uint4 (&t)[3]) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    t[k] = make_uint4(upper2(r[0], r[1]), upper2(r[2], r[3]), upper2(r[4], r[5]), upper2(r[6], r[7]));
+    if (k < 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = drop_upper(r[i]);
+    }
+  }
+}
+
+// 8 int8 codes (two dwords) as bf16, exact.
+__device__ __forceinline__ uint4 codes_bf16(uint32_t lo, uint32_t hi) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = static_cast<float>(static_cast<int8_t>(lo >> (8 * i)));
+    f[4 + i] = static_cast<float>(static_cast<int8_t>(hi >> (8 * i)));
+  }
+  return make_uint4(upper2(f[0], f[1]), upper2(f[2], f[3]), upper2(f[4], f[5]), upper2(f[6], f[7]));
+}
+
+template <bool Q8, int DH>
+struct Tile {
+  static constexpr int NK = Q8 ? DH / 32 : DH / 16;  // 16-byte loads of K, and of V
+  uint4 k[NK], v[NK];
+  float4 ks[Q8 ? 4 : 1], vs[Q8 ? 4 : 1];
+  bool mapped0, mapped1;  // the tile's two blocks
+};
+
+// The dims of k-step s, lane half h, element e: bf16 K is loaded 8 dims at a time, the 8-bit codes
+// 16 at a time, which serve two k-steps.
+template <bool Q8>
+__device__ __forceinline__ int dim_of(int s, int h) {
+  return Q8 ? 32 * (s >> 1) + 16 * h + 8 * (s & 1) : 16 * s + 8 * h;
+}
+
+template <bool Q8, int DH>
+__device__ __forceinline__ void load_tile(Tile<Q8, DH>& t, const SharedArgs& a, int row_b, int kvh,
+                                          int tile, int last_blk, int lane) {
+  const int b0 = min(2 * tile, last_blk), b1 = min(2 * tile + 1, last_blk);
+  const int h = lane >> 5;
+  const bool second = lane & 4;                            // K: the row's block
+  const int at = 4 * ((lane >> 3) & 3) + (lane & 3);       // and its place there
+  if constexpr (Q8) {
+    long n0 = a.map.block(row_b, b0, kvh), n1 = a.map.block(row_b, b1, kvh);
+    t.mapped0 = n0 >= 0;
+    t.mapped1 = n1 >= 0;
+    n0 = max(n0, 0L);  // unmapped: block 0 is read, its keys are masked
+    n1 = max(n1, 0L);
+    const int8_t* k = a.p.kq + ((second ? n1 : n0) * kQ8Block + at) * DH + 16 * h;
+    const long nv = h ? n1 : n0;
+    const int8_t* v = a.p.vq + (nv * DH + (lane & 31)) * kQ8Block;
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i) t.k[i] = *reinterpret_cast<const uint4*>(k + 32 * i);
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i) t.v[i] = *reinterpret_cast<const uint4*>(v + 32 * i * kQ8Block);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      t.ks[i] = *reinterpret_cast<const float4*>(a.p.ks + nv * kQ8Block + 4 * i);
+      t.vs[i] = *reinterpret_cast<const float4*>(a.p.vs + nv * kQ8Block + 4 * i);
+    }
+  } else {
+    const int p0 = a.map.page(row_b, b0), p1 = a.map.page(row_b, b1);
+    t.mapped0 = p0 >= 0;
+    t.mapped1 = p1 >= 0;
+    const int bs = a.map.block_shift, msk = (1 << bs) - 1;
+    const long rs = static_cast<long>(a.p.Hkv) * DH;
+    // row of the block's first key
+    const long r0 = ((static_cast<long>(max(p0, 0)) << bs) + (b0 & msk)) << 4;
+    const long r1 = ((static_cast<long>(max(p1, 0)) << bs) + (b1 & msk)) << 4;
+    const uint16_t* k = a.p.kpool + ((second ? r1 : r0) + at) * rs + kvh * DH + 8 * h;
+#pragma unroll
+    for (int i = 0; i < DH / 16; ++i) t.k[i] = *reinterpret_cast<const uint4*>(k + 16 * i);
+    // V rows as they lie: DH / 8 lanes per row, rows in order
+    constexpr int LPR = DH / 8, RPI = 64 / LPR;  // lanes per row, rows per load
+    const uint16_t* v = a.p.vpool + kvh * DH + 8 * (lane % LPR);
+#pragma unroll
+    for (int i = 0; i < DH / 16; ++i) {
+      const int r = RPI * i;  // a load's rows lie in one block: RPI divides 16
+      t.v[i] = *reinterpret_cast<const uint4*>(v + ((r < 16 ? r0 : r1) + (r & 15) + lane / LPR) * rs);
+    }
+  }
+}
+
+template <int DH>
+constexpr int kVStride = DH + 16;  // bf16 elements of a V row in LDS
+
+template <bool Q8, int DH>
+__global__ __launch_bounds__(64 * kWaves, 1) void shared_attn_kernel(SharedArgs a) {
+  constexpr int NS = DH / 16;  // k-steps of the first product
+  constexpr int ND = DH / 32;  // dim blocks of the second
+  constexpr int OS = DH + 4;   // floats of an output row in LDS
+  constexpr size_t kVBytes = Q8 ? 0 : kTile * kVStride<DH> * 2;
+  constexpr size_t kOBytes = kCols * OS * 4;
+  __shared__ __align__(16) unsigned char smem[kWaves * (kVBytes > kOBytes ? kVBytes : kOBytes)];
+  __shared__ float s_m[kWaves][kCols], s_l[kWaves][kCols];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, col = lane & 31;
+  const int G = a.G, Hq = a.p.Hq, Hkv = a.p.Hkv, P = a.p.shared_len;
+
+  // ---- the unit: its columns, table row and keys [lo, hi) ----
+  const int kvh = blockIdx.x % Hkv;
+  int u = blockIdx.x / Hkv;
+  const int n_prefix = a.col_blocks * a.n_pre;
+  int row_b, lo, hi, slot, b_col, g_col;
+  bool valid;
+  if (u < n_prefix) {
+    const int part = u / a.col_blocks;
+    const int r = (u % a.col_blocks) * kCols + col;
+    b_col = r / G;
+    g_col = r % G;
+    valid = b_col < a.p.B && stream_len(a, min(b_col, a.p.B - 1)) >= P;
+    row_b = 0;
+    lo = part * a.pre_tiles * kTile;
+    hi = min(lo + a.pre_tiles * kTile, P);
+    slot = part;
+  } else {
+    u -= n_prefix;
+    const int part = u % a.n_own;
+    u /= a.n_own;
+    g_col = (u % a.own_chunks) * kCols + col;
+    b_col = u / a.own_chunks;
+    valid = g_col < G;
+    const int S = stream_len(a, b_col);
+    const int first = S < P ? 0 : P;
+    row_b = S < P ? 0 : b_col;
+    // whole tiles, counted from the tile that `first` lies in
+    const int t0 = first / kTile, n = (S + kTile - 1) / kTile - t0;
+    const int per = (n + a.n_own - 1) / a.n_own;
+    lo = max(first, (t0 + part * per) * kTile);
+    hi = min(S, (t0 + (part + 1) * per) * kTile);
+    slot = a.n_pre + part;
+  }
+  if (!valid) b_col = 0, g_col = 0;  // reads an existing row, writes nothing
+
+  float m = -INFINITY, l = 0.0f;
+  f32x16_t o[ND] = {};
+  const int t_end = hi > lo ? (hi + kTile - 1) / kTile : 0;
+  int tile = lo / kTile + wave;
+  const int last_blk = (hi - 1) >> 4;
+  Tile<Q8, DH> nxt;
+  if (tile < t_end) load_tile(nxt, a, row_b, kvh, tile, last_blk, lane);
+
+  // q as three terms: column `col`, the dims of each k-step and half
+  uint4 q[NS][3];
+  const float* qrow = a.p.q + (static_cast<long>(b_col) * Hq + kvh * G + g_col) * DH;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = qrow[dim_of<Q8>(s, h) + e];
+    split3(x, q[s]);
+  }
+  uint16_t* vt = reinterpret_cast<uint16_t*>(smem + wave * kVBytes);
+
+  for (; tile < t_end; tile += kWaves) {
+    const Tile<Q8, DH> cur = nxt;
+    if (tile + kWaves < t_end) load_tile(nxt, a, row_b, kvh, tile + kWaves, last_blk, lane);
+    const int key0 = kTile * tile + 16 * h;  // this lane's 16 keys
+    const bool mapped = h ? cur.mapped1 : cur.mapped0;
+    const bool whole = cur.mapped0 && cur.mapped1 && kTile * tile >= lo && kTile * (tile + 1) <= hi;
+    if constexpr (!Q8) {
+      constexpr int LPR = DH / 8, RPI = 64 / LPR;
+      // rows that are not attended go in as zeros: their weights are 0, and 0 * inf is NaN
+#pragma unroll
+      for (int i = 0; i < DH / 16; ++i) {
+        const int r = RPI * i + lane / LPR, key = kTile * tile + r;
+        const bool in = whole || ((RPI * i < 16 ? cur.mapped0 : cur.mapped1) && key >= lo && key < hi);
+        *reinterpret_cast<uint4*>(vt + r * kVStride<DH> + 8 * (lane % LPR)) =
+            in ? cur.v[i] : make_uint4(0, 0, 0, 0);
+      }
+    }
+    f32x16_t sc = {};
+#pragma unroll
+    for (int k = 2; k >= 0; --k)  // the small terms first
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        uint4 kf;
+        if constexpr (Q8) {
+          const uint4 c = cur.k[s >> 1];
+          kf = (s & 1) ? codes_bf16(c.z, c.w) : codes_bf16(c.x, c.y);
+        } else {
+          kf = cur.k[s];
+        }
+        sc = mfma32(as_bf16x8(kf), as_bf16x8(q[s][k]), sc);
+      }
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i] = sc[i] * a.scale_log2e;
+      if constexpr (Q8) x[i] *= reinterpret_cast<const float*>(cur.ks)[i];
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (!mapped || key0 + i < lo || key0 + i >= hi) x[i] = -INFINITY;
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+    mx = xor32_max(mx);
+    if (__any(mx > m + kSlack)) {  // m is -infinity before the first key
+      const float mn = fmaxf(m, mx);
+      const float ref = mn == -INFINITY ? 0.0f : mn;
+      const float c = fast_exp2(m - ref);
+      l *= c;
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[n][i] *= c;
+      m = mn;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      w[i] = fast_exp2(x[i] - ref);
+      l += w[i];
+      if constexpr (Q8) w[i] *= reinterpret_cast<const float*>(cur.vs)[i];
+    }
+    if (Q8 && !whole) {  // a scale behind the last key may be anything
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (!mapped || key0 + i < lo || key0 + i >= hi) w[i] = 0.0f;
+    }
+    uint4 wt[2][3];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const float y[8] = {w[8 * s],     w[8 * s + 1], w[8 * s + 2], w[8 * s + 3],
+                          w[8 * s + 4], w[8 * s + 5], w[8 * s + 6], w[8 * s + 7]};
+      split3(y, wt[s]);
+    }
+    if constexpr (!Q8) wave_lds_sync();
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        uint4 vf;
+        if constexpr (Q8) {
+          const uint4 c = cur.v[n];
+          vf = s ? codes_bf16(c.z, c.w) : codes_bf16(c.x, c.y);
+        } else {
+          // keys 16 h + 8 s + 0..3 and + 4..7 of dim 32 n + (lane & 31)
+          const uint16_t* at = vt + (16 * h + 8 * s + ((lane & 15) >> 2)) * kVStride<DH> + 32 * n +
+                               (lane & 16) + 4 * (lane & 3);
+          const uint2 x0 = lds_read_tr16(at), x1 = lds_read_tr16(at + 4 * kVStride<DH>);
+          vf = make_uint4(x0.x, x0.y, x1.x, x1.y);
+        }
+#pragma unroll
+        for (int k = 2; k >= 0; --k) o[n] = mfma32(as_bf16x8(vf), as_bf16x8(wt[s][k]), o[n]);
+      }
+    if constexpr (!Q8) wave_lds_sync();  // the tile's buffer is written again
+  }
+
+  // ---- the waves joined in LDS ----
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(smem + wave * kOBytes);
+  l = xor32_sum(l);
+  if (h == 0) {
+    s_m[wave][col] = m;
+    s_l[wave][col] = l;
+  }
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<float4*>(so + col * OS + 32 * n + 8 * r + 4 * h) =
+          make_float4(o[n][4 * r], o[n][4 * r + 1], o[n][4 * r + 2], o[n][4 * r + 3]);
+  __syncthreads();
+  const float* all = reinterpret_cast<const float*>(smem);
+  const bool prefix = blockIdx.x / Hkv < static_cast<unsigned>(n_prefix);
+  for (int i = tid; i < kCols * (DH / 4); i += 64 * kWaves) {
+    const int c = i / (DH / 4), d = 4 * (i % (DH / 4));
+    int b, g;
+    if (prefix) {
+      const int r = static_cast<int>((blockIdx.x / Hkv) % a.col_blocks) * kCols + c;
+      b = r / G;
+      g = r % G;
+      if (b >= a.p.B) continue;
+    } else {
+      const int v = (blockIdx.x / Hkv - n_prefix) / a.n_own;
+      g = (v % a.own_chunks) * kCols + c;
+      b = v / a.own_chunks;
+      if (g >= G) continue;
+    }
+    float M = -INFINITY, L = 0.0f;
+    float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, s_m[w][c]);
+    // a stream that is no column of the prefix leaves nothing there
+    const bool none = prefix && stream_len(a, b) < P;
+    const float ref = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = fast_exp2(s_m[w][c] - ref);
+      const float4 x = *reinterpret_cast<const float4*>(all + w * (kOBytes / 4) + c * OS + d);
+      L = fmaf(f, s_l[w][c], L);
+      r.x = fmaf(f, x.x, r.x);
+      r.y = fmaf(f, x.y, r.y);
+      r.z = fmaf(f, x.z, r.z);
+      r.w = fmaf(f, x.w, r.w);
+    }
+    const long ps = (static_cast<long>(b) * Hq + kvh * G + g) * a.slots + slot;
+    if (none) {
+      M = -INFINITY;
+      L = 0.0f;
+      r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    *reinterpret_cast<float4*>(a.part_o + ps * DH + d) = r;
+    if (d == 0) {
+      a.part_ml[2 * ps] = M;
+      a.part_ml[2 * ps + 1] = L;
+    }
+  }
+}
+
+// One wave per (stream, head): out = sum_j 2^(m_j - M) o_j / sum_j 2^(m_j - M) l_j over its slots.
+template <int DH>
+__global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
+  const int lane = threadIdx.x & 63;
+  const long row = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= static_cast<long>(a.p.B) * a.p.Hq) return;
+  constexpr int E = DH / 64;
+  float M = -INFINITY, L = 0.0f, o[E] = {};
+  for (int s0 = 0; s0 < a.slots; s0 += 64) {
+    const bool in = s0 + lane < a.slots;
+    const long ps = row * a.slots + s0 + lane;
+    const float m = in ? a.part_ml[2 * ps] : -INFINITY;
+    const float l = in ? a.part_ml[2 * ps + 1] : 0.0f;
+    const float mn = fmaxf(M, wave_max(m));
+    const float ref = mn == -INFINITY ? 0.0f : mn;
+    const float c = fast_exp2(M - ref), w = fast_exp2(m - ref);
+    M = mn;
+    L = fmaf(L, c, wave_sum(w * l));
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= c;
+    const int n = min(64, a.slots - s0);
+    for (int j = 0; j < n; ++j) {
+      const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        o[e] = fmaf(wj, a.part_o[(row * a.slots + s0 + j) * DH + 64 * e + lane], o[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    a.p.out[row * DH + 64 * e + lane] = L == 0.0f ? 0.0f : o[e] / L;
+}
+
+template <bool Q8, int DH>
+int launch(const SharedArgs& a, unsigned grid, hipStream_t stream) {
+  hipLaunchKernelGGL((shared_attn_kernel<Q8, DH>), dim3(grid), dim3(64 * kWaves), 0, stream, a);
+  if (int rc = check_launch("shared_attn_kernel")) return rc;
+  const long rows = static_cast<long>(a.p.B) * a.p.Hq;
+  hipLaunchKernelGGL((shared_merge_kernel<DH>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0,
+                     stream, a);
+  return check_launch("shared_merge_kernel");
+}
+
+}  // namespace
+
+int launch_shared_prefix(const KeysProblem& p, const Q8Map& map, hipStream_t stream) {
+  SharedArgs a{};
+  a.p = p;
+  a.map = map;
+  a.scale_log2e = p.scale * 1.4426950408889634f;
+  a.G = p.Hq / p.Hkv;
+  const long rows = static_cast<long>(p.B) * a.G;
+  a.col_blocks = static_cast<int>((rows + kCols - 1) / kCols);
+  a.own_chunks = (a.G + kCols - 1) / kCols;
+  const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
+  // one workgroup per CU for each kind of unit, each of at least one tile per wave
+  const long tiles = (p.shared_len + kTile - 1) / kTile;
+  const long pre_units = static_cast<long>(a.col_blocks) * p.Hkv;
+  long n_pre = tiles == 0 ? 0 : std::clamp(cus / pre_units, 1L, (tiles + kWaves - 1) / kWaves);
+  a.pre_tiles = n_pre ? static_cast<int>((tiles + n_pre - 1) / n_pre) : 0;
+  a.n_pre = a.pre_tiles ? static_cast<int>((tiles + a.pre_tiles - 1) / a.pre_tiles) : 0;
+  const long own = (static_cast<long>(map.capacity) - p.shared_len + kTile - 1) / kTile + 1;
+  const long own_units = static_cast<long>(p.B) * p.Hkv * a.own_chunks;
+  a.n_own = static_cast<int>(std::clamp(cus / own_units, 1L, (own + kWaves - 1) / kWaves));
+  a.slots = a.n_pre + a.n_own;
+  const long grid = pre_units * a.n_pre + own_units * a.n_own;
+  if (grid > 0x7fffffffL)
+    return fail(ORATOR_ERR_UNSUPPORTED, "gqa_decode_shared: too many streams and heads");
+  const size_t parts = static_cast<size_t>(p.B) * p.Hq * a.slots;
+  char* ws = static_cast<char*>(workspace_graph(stream, parts * (p.Dh + 2) * sizeof(float), kWsKeys));
+  if (!ws) return ORATOR_ERR_HIP;
+  a.part_o = reinterpret_cast<float*>(ws);
+  a.part_ml = a.part_o + parts * p.Dh;
+  const unsigned g = static_cast<unsigned>(grid);
+  if (p.bf16) return p.Dh == 128 ? launch<false, 128>(a, g, stream) : launch<false, 64>(a, g, stream);
+  return p.Dh == 128 ? launch<true, 128>(a, g, stream) : launch<true, 64>(a, g, stream);
+}
+
+}  // namespace orator_hip
