@@ -34,6 +34,7 @@ constexpr int kWsPrefillArrive = 5;  // its arrival counters
 constexpr int kWsKeys = 6;       // partials of the 8-bit cache's and the shared prefix's attention
 constexpr int kWsKeysArrive = 8;  // their arrival counters
 constexpr int kWsLogprobs = 7;   // partials of the token log probabilities
+constexpr int kWsLogprobsArrive = 9;
 // *fresh (optional): the block was allocated by this call, its contents undefined.
 void* workspace(hipStream_t stream, size_t bytes, int slot = 0, bool* fresh = nullptr);
 // workspace() for the operators whose captured calls need no reserve call before the capture: while
