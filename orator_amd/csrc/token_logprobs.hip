@@ -4,15 +4,19 @@
 //   lse = m + log S,  logprob = x_tok - lse,  entropy = log S - T / S.
 // Entries of -infinity have weight 0 and add 0 to T.
 //
-// Memory-bound: the logits are read once.  A row is cut into parts of up to 8192 entries, one
-// workgroup each, which holds its part in registers (32 entries a thread): the maximum, the sums
-// against it, and the part's best entries, all from the one read.  The last workgroup of a row to
-// finish joins its parts.
+// Memory-bound: the logits are read once.  A row is cut into parts, one workgroup each, and a part
+// into chunks of up to 4096 entries that a workgroup holds in registers (16 a thread) while the next
+// one is loaded.  Every thread keeps its own maximum and sums; nothing is exchanged between chunks.
+// The last workgroup of a row to finish joins its parts.
 //
-// Best entries of a part: the k-th largest of the 64 lanes' maxima of a wave is a bound that k
-// entries reach; entries at or above the largest of the waves' bounds (k to a few hundred) go to
-// LDS, and each finds its rank by counting those before it.  Parts where that leaves too many (ties
-// in masses) or too few (NaN) extract their best one after the other instead.
+// Best entries: a wave keeps a list in LDS of entries that may be among the k best of its own.  The
+// k-th largest of the 64 lanes' running maxima is a bound that k entries reach, so entries below it
+// are left out (1024 entries of a wave add some 24 at first, then ever fewer).  A chunk with too many (ties
+// in masses) gives its k best one after the other instead; a full list is cut to its k best.  What
+// the waves listed is ranked by counting, per part and then per row.  Entries of -infinity and NaN
+// are never listed: a row with fewer than k others is searched for them at the end.
+#include <float.h>
+
 #include <algorithm>
 #include <string>
 
@@ -25,12 +29,16 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kTopMax = 32;
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kThreads = 256;
 constexpr int kWavesN = kThreads / 64;
-constexpr int kVec = 8;                           // float4 per thread
-constexpr int kPart = kThreads * kVec * 4;        // entries of a part, at most
-constexpr int kCand = 768;                        // candidates kept in LDS
-constexpr int kFirst = 256;                       // entries whose -infinity may be a candidate
+constexpr int kVec = 4;                           // float4 per thread and chunk
+constexpr int kChunk = kThreads * kVec * 4;       // entries of a chunk, at most
+constexpr int kList = 192;                        // a wave's list
+constexpr int kFew = 6;                           // lanes with entries to list that need no new bound
+constexpr int kMost = 96;                         // entries that one chunk may add to it
+constexpr int kCand = 768;                        // candidates ranked at once
+static_assert(kTopMax + kMost <= kList && kWavesN * kList <= kCand && kTopMax <= 64);
 
 struct LogprobArgs {
   const float* x;
@@ -41,7 +49,7 @@ struct LogprobArgs {
   float* entropy;
   int* top_ids;
   float* top_logprobs;
-  int parts, part_len;
+  int parts, chunks, chunk_len;  // chunks of chunk_len entries (a multiple of 4) per part
   float* stats;      // [rows][parts][4]: m, S, T
   u64* best;         // [rows][parts][top_k], descending; 0: none
   unsigned* arrive;  // [rows], kCounterStride apart; null: one part
@@ -96,153 +104,286 @@ struct RowSums {
   }
 };
 
-__global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a) {
-  __shared__ float s_red[kWavesN][3];
-  __shared__ uint32_t s_bound[kWavesN];
-  __shared__ u64 s_cand[kCand];
-  __shared__ u64 s_best[kTopMax];
-  __shared__ int s_n, s_inf, s_last;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int part = blockIdx.x % a.parts;
-  const int row = blockIdx.x / a.parts;
-  const float* x = a.x + row * a.row_stride;
-  const int base = part * a.part_len;
-  const int n = min(a.part_len, a.vocab - base);  // >= 1
-  const int k = a.top_k;
+// v >= above(t) says v > t.
+__device__ __forceinline__ float above(float t) { return value_of(order_of(t) + 1u); }
 
-  // ---- the part, 4 consecutive entries at (i * kThreads + tid) * 4; behind its end -infinity ----
-  float v[kVec][4];
+// Writes the keys of list[0, n) that are among its k largest (all of them, if fewer) to best[0, k),
+// in order, 0 behind them; `threads` threads take part, this one is number t.  List and best apart.
+__device__ __forceinline__ void rank_into(u64* best, const u64* list, int n, int k, int t, int threads) {
+  for (int c = t; c < n; c += threads) {
+    const u64 key = list[c];
+    int rank = 0, o = 0;
+    for (; o + 8 <= n; o += 8) {  // eight reads on the way at a time
+      u64 other[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) other[i] = list[o + i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rank += other[i] > key ? 1 : 0;
+    }
+    for (; o < n; ++o) rank += list[o] > key ? 1 : 0;
+    if (rank < k) best[rank] = key;
+  }
+  if (t < k && t >= n) best[t] = 0;
+}
+
+typedef float Chunk[kVec][4];
+
+// Chunk entries (i * kThreads + tid) * 4 + j of n, as loaded: a group of four that does not lie in
+// the chunk holds its last four entries (chunks of fewer than 4: none), which finish_chunk puts right
+// once they are there.  No branch stands between the loads.
+__device__ __forceinline__ void load_chunk(Chunk& v, const float* x, int n, int tid) {
+  if (n < 4) return;  // uniform
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
-    const int at = (i * kThreads + tid) * 4;
-    if (at + 4 <= n) {
-      const Vec4 r = load4(x + base + at);
+    const Vec4 r = load4(x + min((i * kThreads + tid) * 4, n - 4));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = r.v[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = at + j < n ? x[base + at + j] : -INFINITY;
-    }
+    for (int j = 0; j < 4; ++j) v[i][j] = r.v[j];
   }
-  if (tid == 0) s_n = s_inf = 0;
-
-  // ---- maximum, bound of the k-th best, sums ----
-  float mine = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kVec; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) mine = fmaxf(mine, v[i][j]);
-  const float wm = wave_max(mine);
-  uint32_t bound = 0;
-  if (k > 0) {
-    // the upper 16 bits of the largest number that k lanes' maxima reach
-    const uint32_t o = order_of(mine);
-    for (int bit = 31; bit >= 16; --bit) {
-      const uint32_t t = bound | 1u << bit;
-      if (__popcll(__ballot(o >= t)) >= k) bound = t;
-    }
-  }
-  if (lane == 0) {
-    s_red[wave][0] = wm;
-    s_bound[wave] = bound;
-  }
-  __syncthreads();
-  float m = s_red[0][0];
-  uint32_t limit = s_bound[0];
-#pragma unroll
-  for (int w = 1; w < kWavesN; ++w) {
-    m = fmaxf(m, s_red[w][0]);
-    limit = max(limit, s_bound[w]);
-  }
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float S = 0.0f, T = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kVec; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float d = v[i][j] - ref;
-      const float e = fast_exp2(d * 1.4426950408889634f);
-      S += e;
-      T += d == -INFINITY ? 0.0f : e * d;
-    }
-  S = wave_sum(S);
-  T = wave_sum(T);
-  __syncthreads();  // s_red is read
-  if (lane == 0) {
-    s_red[wave][1] = S;
-    s_red[wave][2] = T;
-  }
-
-  // ---- the part's best entries ----
-  if (k > 0) {
-    // Entries that may be among the best: at or above the limit.  A limit that -infinity reaches
-    // says nothing: then every number, and the -infinity entries among the first kFirst, which are
-    // enough of them if they are k (ids count upwards).
-    const bool low = limit <= order_of(-INFINITY);
-    const float lim = low ? -INFINITY : value_of(limit);
+}
+// Entries behind the chunk's end become -infinity.
+__device__ __forceinline__ void finish_chunk(Chunk& v, const float* x, int n, int tid) {
+  if (n == kChunk) return;  // uniform
+  if (n < 4) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = (i * kThreads + tid) * 4 + j;
-        const bool inf = low && at < min(n, kFirst) && v[i][j] == -INFINITY;
-        if (low ? inf || v[i][j] > lim : v[i][j] >= lim) {
-          const int slot = atomicAdd(&s_n, 1);
-          if (slot < kCand) s_cand[slot] = key_of(v[i][j], base + at);
-          if (inf) atomicAdd(&s_inf, 1);
-        }
-      }
-    __syncthreads();
-    const int want = min(k, n);
-    const int found = s_n;
-    if (found >= want && found <= kCand && (!low || s_inf >= k || n <= kFirst)) {
-      for (int c = tid; c < found; c += kThreads) {
-        const u64 key = s_cand[c];
-        int rank = 0;
-        for (int o = 0; o < found; ++o) rank += s_cand[o] > key ? 1 : 0;
-        if (rank < k) s_best[rank] = key;
-      }
-      if (tid < k && tid >= found) s_best[tid] = 0;
-    } else {
-      // one after the other: each wave takes its own largest entry below its last one
-      __syncthreads();
-      u64 last = ~0ull;
-      for (int r = 0; r < k; ++r) {
-        u64 top = 0;
+      for (int j = 0; j < 4; ++j) v[i][j] = i == 0 && tid == 0 && j < n ? x[j] : -INFINITY;
+    return;
+  }
 #pragma unroll
-        for (int i = 0; i < kVec; ++i)
+  for (int i = 0; i < kVec; ++i) {
+    if ((i + 1) * kThreads * 4 <= n) continue;  // uniform
+    const int past = (i * kThreads + tid) * 4 - (n - 4);  // entries that the load came too early
+    if (past > 0) {
+      v[i][0] = past == 1 ? v[i][1] : past == 2 ? v[i][2] : past == 3 ? v[i][3] : -INFINITY;
+      v[i][1] = past == 1 ? v[i][2] : past == 2 ? v[i][3] : -INFINITY;
+      v[i][2] = past == 1 ? v[i][3] : -INFINITY;
+      v[i][3] = -INFINITY;
+    }
+  }
+}
+
+// A thread's sums over its entries so far; T in units of log 2, as the exponents are.
+struct Sums {
+  float m = -INFINITY, S = 0.0f, T = 0.0f;
+
+  // To a maximum of m2 >= m.  d may be as large as the type's lowest value makes it: a weight of 0
+  // leaves nothing (0 * inf is NaN); S keeps a NaN.
+  __device__ __forceinline__ void move(float m2) {
+    if (m2 == -INFINITY) return;
+    const float t = m == -INFINITY ? 0.0f : (m - m2) * kLog2e;
+    const float c = fast_exp2(t);
+    T = c == 0.0f ? 0.0f : c * fmaf(t, S, T);
+    S *= c;
+    m = m2;
+  }
+  __device__ __forceinline__ void take(float x, float ref) {
+    const float t = (x - ref) * kLog2e;
+    const float e = fast_exp2(t);
+    S += e;
+    T = fmaf(e, fmaxf(t, -FLT_MAX), T);  // a weight of 0 leaves 0; S keeps a NaN
+  }
+};
+
+// A wave's list of entries that may be among its k best.
+struct List {
+  u64* at;              // kList in LDS
+  int n = 0;            // uniform
+  float thr = -FLT_MAX; // entries below are not listed (NaN: none is)
+  float reach = -INFINITY;  // k listed entries reach this
+  float lane_max = -INFINITY;
+
+  __device__ __forceinline__ void add(bool in, u64 key) {
+    const u64 mask = __ballot(in);
+    if (mask == 0) return;
+    const int slot = n + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                                   __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+    if (in) at[slot] = key;
+    n += __popcll(mask);
+  }
+
+  // The list cut to its k best (it has at least k); later entries have to be above the last.
+  __device__ __forceinline__ void cut(int k, int lane) {
+    wave_lds_sync();
+    constexpr int N = kList / 64;
+    u64 mine[N];
+    int rank[N] = {};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int at = (i * kThreads + tid) * 4 + j;
-            const u64 key = at < n ? key_of(v[i][j], base + at) : 0;
-            if (key < last) top = max64(top, key);
-          }
-        last = wave_max64(top);
-        if (lane == 0) s_cand[wave * kTopMax + r] = last;
+    for (int i = 0; i < N; ++i) mine[i] = 64 * i + lane < n ? at[64 * i + lane] : 0;
+    for (int o = 0; o < n; ++o) {
+      const u64 key = at[o];
+#pragma unroll
+      for (int i = 0; i < N; ++i) rank[i] += key > mine[i] ? 1 : 0;
+    }
+    wave_lds_sync();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (64 * i + lane < n && rank[i] < k) at[rank[i]] = mine[i];
+    wave_lds_sync();
+    n = k;
+    reach = value_of(static_cast<uint32_t>(at[k - 1] >> 32));
+    thr = above(reach);
+  }
+
+  // The chunk's entries, their ids from id0 on, all higher than those listed.
+  // m4: the maxima of the lane's groups of four; chunk_max: of all.
+  __device__ __forceinline__ void take(const Chunk& v, const float (&m4)[kVec], float chunk_max,
+                                       int id0, int k, int tid, int lane) {
+    lane_max = fmaxf(lane_max, chunk_max);
+    const int lanes = __popcll(__ballot(chunk_max >= thr));
+    if (lanes == 0) return;
+    if (lanes > kFew) {
+      // the upper 16 bits of the largest number that k lanes' maxima reach
+      const uint32_t o = order_of(lane_max);
+      uint32_t bound = 0;
+#pragma unroll
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t t = bound | 1u << bit;
+        if (__popcll(__ballot(o >= t)) >= k) bound = t;
       }
-      if (tid < kTopMax) s_best[tid] = 0;
-      __syncthreads();
-      if (lane < k) {
-        const u64 key = s_cand[wave * kTopMax + lane];
-        int rank = 0;
-        for (int w = 0; w < kWavesN; ++w)
-          for (int r = 0; r < k; ++r) rank += s_cand[w * kTopMax + r] > key ? 1 : 0;
-        if (key != 0 && rank < k) s_best[rank] = key;
+      if (bound > order_of(-INFINITY)) {
+        const float b = value_of(bound);
+        // k of the wave's entries so far reach b, and those that do are listed or in this chunk
+        if (b > reach) reach = b;
+        if (b > thr) thr = b;
       }
     }
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) count += 4 * __popcll(__ballot(m4[i] >= thr));
+    if (count > kMost) {  // at most that many: count them
+      count = 0;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) count += __popcll(__ballot(v[i][j] >= thr));
+      if (count > kMost) {
+        best_of(v, id0, k, tid, lane);
+        return;
+      }
+    }
+    if (n + count > kList) cut(k, lane);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      if (__ballot(m4[i] >= thr) == 0) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        add(v[i][j] >= thr, key_of(v[i][j], id0 + (i * kThreads + tid) * 4 + j));
+    }
+  }
+
+  // The k best of a chunk that has more than kMost to list, one after the other.
+  __device__ __forceinline__ void best_of(const Chunk& v, int id0, int k, int tid, int lane) {
+    if (n + k > kList) cut(k, lane);
+    u64 last = ~0ull;
+    for (int r = 0; r < k; ++r) {
+      u64 top = 0;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float y = v[i][j];
+          asm volatile("" : "+v"(y));  // keys formed in the loop: 32 held across it are 64 registers
+          const u64 key = key_of(y, id0 + (i * kThreads + tid) * 4 + j);
+          if (y >= thr && key < last) top = max64(top, key);
+        }
+      last = wave_max64(top);
+      if (lane == 0) at[n + r] = last;
+    }
+    n += k;
+    cut(k, lane);
+  }
+};
+
+__global__ __launch_bounds__(kThreads, 5) void token_logprobs_kernel(LogprobArgs a) {
+  __shared__ float s_sums[kWavesN][3];
+  __shared__ float s_reach[kWavesN];
+  __shared__ u64 s_list[kWavesN][kList];
+  __shared__ u64 s_cand[kCand];
+  __shared__ u64 s_best[kTopMax];
+  __shared__ int s_len[kWavesN], s_n, s_last;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = blockIdx.x % a.parts;
+  const int row = blockIdx.x / a.parts;
+  const float* x = a.x + row * a.row_stride;
+  const int k = a.top_k;
+  const long base = static_cast<long>(part) * a.chunks * a.chunk_len;
+  x += base;
+  // the part's entries (none for a part behind the row's end)
+  const int entries = static_cast<int>(
+      max(0L, min(static_cast<long>(a.chunks) * a.chunk_len, a.vocab - base)));
+  Sums sum;
+  List list;
+  list.at = s_list[wave];
+  Chunk nxt = {};
+  load_chunk(nxt, x, min(a.chunk_len, entries), tid);
+  for (int c0 = 0; c0 < entries; c0 += a.chunk_len) {
+    const int n = min(a.chunk_len, entries - c0);
+    Chunk v;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = nxt[i][j];
+    load_chunk(nxt, x + c0 + a.chunk_len, min(a.chunk_len, entries - c0 - a.chunk_len), tid);
+    finish_chunk(v, x + c0, n, tid);
+    float m4[kVec], mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      m4[i] = fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3]));
+      mx = fmaxf(mx, m4[i]);
+    }
+    if (mx > sum.m) sum.move(mx);
+    const float ref = sum.m == -INFINITY ? 0.0f : sum.m;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum.take(v[i][j], ref);
+    if (k > 0) list.take(v, m4, mx, static_cast<int>(base) + c0, k, tid, lane);
+  }
+
+  x -= base;
+
+  // ---- the part's sums and best entries ----
+  sum.move(wave_max(sum.m));
+  sum.S = wave_sum(sum.S);
+  sum.T = wave_sum(sum.T);
+  if (lane == 0) {
+    s_sums[wave][0] = sum.m, s_sums[wave][1] = sum.S, s_sums[wave][2] = sum.T;
+    s_reach[wave] = list.reach;
+    s_len[wave] = list.n;
+  }
+  if (tid == 0) s_n = 0;
+  __syncthreads();
+  if (k > 0) {
+    float reach = s_reach[0];
+#pragma unroll
+    for (int w = 1; w < kWavesN; ++w) reach = fmaxf(reach, s_reach[w]);
+    const uint32_t lim = order_of(reach);
+    for (int w = 0; w < kWavesN; ++w)
+      for (int c = tid; c < s_len[w]; c += kThreads) {
+        const u64 key = s_list[w][c];
+        if (static_cast<uint32_t>(key >> 32) >= lim) s_cand[atomicAdd(&s_n, 1)] = key;
+      }
+    __syncthreads();
+    rank_into(s_best, s_cand, s_n, k, tid, kThreads);
   }
   __syncthreads();
   const long slot = static_cast<long>(row) * a.parts + part;
   if (tid < k) store_dev(a.best + slot * k + tid, s_best[tid]);
   if (tid == 0) {
-    S = T = 0.0f;
+    Sums p;
     for (int w = 0; w < kWavesN; ++w) {
-      S += s_red[w][1];
-      T += s_red[w][2];
+      Sums q{s_sums[w][0], s_sums[w][1], s_sums[w][2]};
+      const float M = fmaxf(p.m, q.m);
+      p.move(M);
+      q.move(M);
+      p.S += q.S;
+      p.T += q.T;
     }
-    store_dev(a.stats + 4 * slot, m);
-    store_dev(a.stats + 4 * slot + 1, S);
-    store_dev(a.stats + 4 * slot + 2, T);
+    store_dev(a.stats + 4 * slot, p.m);
+    store_dev(a.stats + 4 * slot + 1, p.S);
+    store_dev(a.stats + 4 * slot + 2, p.T);
   }
 
   // ---- the last workgroup of the row joins the parts ----
@@ -261,84 +402,131 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
   __syncthreads();
   if (!s_last) return;
   const float* stats = a.stats + static_cast<long>(row) * a.parts * 4;
-  RowSums sum;
-  float M = -INFINITY;
-  for (int p = lane; p < a.parts; p += 64) M = fmaxf(M, load_dev(stats + 4 * p));
-  M = wave_max(M);
-  sum.ref = M == -INFINITY ? 0.0f : M;
-  sum.S = sum.T = 0.0f;
-  for (int p = lane; p < a.parts; p += 64) {
-    const float mp = load_dev(stats + 4 * p);
-    const float Sp = load_dev(stats + 4 * p + 1), Tp = load_dev(stats + 4 * p + 2);
-    const float d = mp == -INFINITY ? 0.0f : mp - sum.ref;  // a part of -infinity: S = T = 0
-    const float c = fast_exp2(d * 1.4426950408889634f);
-    sum.S = fmaf(c, Sp, sum.S);
-    // weight 0: d may be as large as the type's lowest value makes it, and 0 * inf is NaN
-    sum.T += c == 0.0f ? 0.0f : c * fmaf(d, Sp, Tp);
+  const u64* best = a.best + static_cast<long>(row) * a.parts * k;
+  const long keys = static_cast<long>(a.parts) * k;
+  // everything that is read is on its way before any of it is waited for (parts up to 64, and
+  // kHeld keys a thread; what there is beyond is read in the loops)
+  constexpr int kHeld = 4;
+  u64 held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    held[i] = tid + i * kThreads < keys ? load_dev(best + tid + i * kThreads) : 0;
+  Sums mine;
+  if (lane < a.parts) {
+    mine.m = load_dev(stats + 4 * lane);
+    mine.S = load_dev(stats + 4 * lane + 1);
+    mine.T = load_dev(stats + 4 * lane + 2);
   }
-  sum.S = wave_sum(sum.S);
-  sum.T = wave_sum(sum.T);
-  sum.logS = logf(sum.S);
+  const int token = a.logprob ? a.tokens[row] : -1;
+  const bool known = token >= 0 && token < a.vocab;
+  const float picked = known ? x[token] : 0.0f;
+  float M = mine.m;
+  for (int p = 64 + lane; p < a.parts; p += 64) M = fmaxf(M, load_dev(stats + 4 * p));
+  M = wave_max(M);
+  mine.move(M);
+  Sums all = mine;
+  for (int p = 64 + lane; p < a.parts; p += 64) {
+    Sums q;
+    q.m = load_dev(stats + 4 * p);
+    q.S = load_dev(stats + 4 * p + 1);
+    q.T = load_dev(stats + 4 * p + 2);
+    q.move(M);
+    all.S += q.S;
+    all.T += q.T;
+  }
+  RowSums sums;
+  sums.ref = M == -INFINITY ? 0.0f : M;
+  sums.S = wave_sum(all.S);
+  sums.T = wave_sum(all.T);
+  sums.logS = logf(sums.S);
   if (tid == 0) {
-    if (a.logprob) {
-      const int t = a.tokens[row];
-      a.logprob[row] = t >= 0 && t < a.vocab ? sum.logp(x[t]) : __uint_as_float(0x7fc00000u);
-    }
-    if (a.entropy) a.entropy[row] = sum.S == 0.0f ? 0.0f : sum.logS - sum.T / sum.S;
+    if (a.logprob) a.logprob[row] = known ? sums.logp(picked) : __uint_as_float(0x7fc00000u);
+    if (a.entropy)
+      a.entropy[row] = sums.S == 0.0f ? 0.0f : sums.logS - sums.T * 0.69314718055994531f / sums.S;
   }
   if (k == 0) return;
-  // the best of the parts' k best: those at or above the largest k-th of a part, by rank
-  const u64* best = a.best + static_cast<long>(row) * a.parts * k;
-  u64 floor_key = 0;
-  for (int p = lane; p < a.parts; p += 64) floor_key = max64(floor_key, load_dev(best + p * k + k - 1));
-  floor_key = wave_max64(floor_key);
-  if (floor_key == 0) floor_key = 1;  // parts of fewer than k entries
-  for (int c = tid; c < a.parts * k; c += kThreads) {
-    const u64 key = load_dev(best + c);
-    if (key >= floor_key) {
-      const int at = atomicAdd(&s_n, 1);
-      if (at < kCand) s_cand[at] = key;
-    }
-  }
-  __syncthreads();
-  const int found = s_n;
   int* ids = a.top_ids + static_cast<long>(row) * k;
   float* top = a.top_logprobs + static_cast<long>(row) * k;
+  // the best of the parts' k best: those at or above the largest k-th of a part, by rank
+  u64 lowest = 1;  // 0 stands behind the entries of a part that has fewer than k
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if ((tid + i * kThreads) % k == k - 1) lowest = max64(lowest, held[i]);
+  for (long c = tid + kHeld * kThreads; c < keys; c += kThreads)
+    if (c % k == k - 1) lowest = max64(lowest, load_dev(best + c));
+  lowest = wave_max64(lowest);
+  if (lane == 0) s_list[0][wave] = lowest;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWavesN; ++w) lowest = max64(lowest, s_list[0][w]);
+  auto keep = [&](u64 key) {
+    if (key < lowest) return;
+    const int at = atomicAdd(&s_n, 1);
+    if (at < kCand) s_cand[at] = key;
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) keep(held[i]);
+  for (long c = tid + kHeld * kThreads; c < keys; c += kThreads) keep(load_dev(best + c));
+  __syncthreads();
+  const int found = s_n;
   if (found <= kCand) {
-    for (int c = tid; c < found; c += kThreads) {
-      const u64 key = s_cand[c];
-      int rank = 0;
-      for (int o = 0; o < found; ++o) rank += s_cand[o] > key ? 1 : 0;
-      if (rank < k) {
-        ids[rank] = id_of(key);
-        top[rank] = sum.logp(value_of(static_cast<uint32_t>(key >> 32)));
-      }
+    rank_into(s_best, s_cand, found, k, tid, kThreads);
+    __syncthreads();
+    if (tid < min(k, found)) {
+      const u64 key = s_best[tid];
+      ids[tid] = id_of(key);
+      top[tid] = sums.logp(value_of(static_cast<uint32_t>(key >> 32)));
     }
   } else if (wave == 0) {  // many parts whose best lie close together
     u64 last = ~0ull;
     for (int r = 0; r < k; ++r) {
       u64 t = 0;
-      for (int c = lane; c < a.parts * k; c += 64) {
+      for (long c = lane; c < static_cast<long>(a.parts) * k; c += 64) {
         const u64 key = load_dev(best + c);
         if (key < last) t = max64(t, key);
       }
       last = wave_max64(t);
       if (lane == 0) {
         ids[r] = id_of(last);
-        top[r] = sum.logp(value_of(static_cast<uint32_t>(last >> 32)));
+        top[r] = sums.logp(value_of(static_cast<uint32_t>(last >> 32)));
       }
     }
   }
+  if (found >= k || wave != 0) return;
+  // fewer than k numbers above -infinity: the first entries of -infinity, then the first NaN
+  int r = found;
+  for (int nan = 0; nan < 2 && r < k; ++nan)
+    for (long c = 0; c < a.vocab && r < k; c += 64) {
+      const float y = c + lane < a.vocab ? x[c + lane] : 0.0f;
+      const bool in = nan ? y != y : y == -INFINITY;
+      const u64 mask = __ballot(in);
+      const int at = r + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                                   __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+      if (in && at < k) {
+        ids[at] = static_cast<int>(c + lane);
+        top[at] = sums.logp(y);
+      }
+      r += __popcll(mask);
+    }
 }
 
 // Rows per launch: counters and a workspace of some 32 MB.
 constexpr size_t kSlabBytes = size_t{32} << 20;
 
 int token_logprobs(LogprobArgs a, int rows, hipStream_t stream) {
-  const long parts = (static_cast<long>(a.vocab) + kPart - 1) / kPart;
-  a.parts = static_cast<int>(parts);
-  a.part_len = static_cast<int>(((a.vocab + parts - 1) / parts + 3) / 4 * 4);
-  a.parts = static_cast<int>((static_cast<long>(a.vocab) + a.part_len - 1) / a.part_len);
+  // Parts of a row: the fewest rounds of workgroups (five to a CU) times chunks each, where a
+  // workgroup's start and end cost about as much as two chunks.
+  const long slots = 5L * (device_cu_count() > 0 ? device_cu_count() : 256);
+  const long chunks = (static_cast<long>(a.vocab) + kChunk - 1) / kChunk;
+  long parts = 1, least = 0;
+  for (long p = 1; p <= std::min(chunks, slots); ++p) {
+    const long cost = (rows * p + slots - 1) / slots * ((chunks + p - 1) / p + 2);
+    if (p == 1 || cost < least) least = cost, parts = p;
+  }
+  a.chunks = static_cast<int>((chunks + parts - 1) / parts);
+  a.parts = static_cast<int>((chunks + a.chunks - 1) / a.chunks);
+  const long all = static_cast<long>(a.chunks) * a.parts;
+  a.chunk_len = static_cast<int>(((a.vocab + all - 1) / all + 3) / 4 * 4);
   const size_t per_row = static_cast<size_t>(a.parts) * (4 * sizeof(float) + a.top_k * sizeof(u64));
   const int slab = static_cast<int>(
       std::clamp<size_t>(kSlabBytes / per_row, 1, static_cast<size_t>(std::min(rows, kArriveCounters))));
