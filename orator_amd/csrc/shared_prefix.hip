@@ -145,26 +145,33 @@ __device__ __forceinline__ void load_tile(Tile<Q8, DH>& t, const SharedArgs& a, 
     for (int i = 0; i < DH / 16; ++i) t.k[i] = *reinterpret_cast<const uint4*>(k + 16 * i);
     // V rows as they lie: DH / 8 lanes per row, rows in order
     constexpr int LPR = DH / 8, RPI = 64 / LPR;  // lanes per row, rows per load
-    const uint16_t* v = a.p.vpool + kvh * DH + 8 * (lane % LPR);
+    const uint32_t off = static_cast<uint32_t>(lane / LPR) * static_cast<uint32_t>(rs) + 8 * (lane % LPR);
 #pragma unroll
     for (int i = 0; i < DH / 16; ++i) {
-      const int r = RPI * i;  // a load's rows lie in one block: RPI divides 16
-      t.v[i] = *reinterpret_cast<const uint4*>(v + ((r < 16 ? r0 : r1) + (r & 15) + lane / LPR) * rs);
+      const int r = RPI * i;  // a load's rows lie in one block (RPI divides 16): a uniform base
+      const uint16_t* v = a.p.vpool + ((r < 16 ? r0 : r1) + (r & 15)) * rs + kvh * DH;
+      t.v[i] = *reinterpret_cast<const uint4*>(v + off);
     }
   }
 }
 
 template <int DH>
 constexpr int kVStride = DH + 16;  // bf16 elements of a V row in LDS
+template <int DH>
+constexpr int kQStride = DH + 8;   // and of a q row
 
 template <bool Q8, int DH>
-__global__ __launch_bounds__(64 * kWaves, 1) void shared_attn_kernel(SharedArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs a) {
   constexpr int NS = DH / 16;  // k-steps of the first product
   constexpr int ND = DH / 32;  // dim blocks of the second
   constexpr int OS = DH + 4;   // floats of an output row in LDS
+  constexpr size_t kQTerm = kCols * kQStride<DH>;  // elements of a term of q
+  constexpr size_t kQBytes = 3 * kQTerm * 2;
   constexpr size_t kVBytes = Q8 ? 0 : kTile * kVStride<DH> * 2;
   constexpr size_t kOBytes = kCols * OS * 4;
-  __shared__ __align__(16) unsigned char smem[kWaves * (kVBytes > kOBytes ? kVBytes : kOBytes)];
+  // q's terms and the waves' V tiles; then the waves' outputs
+  constexpr size_t kWork = kQBytes + kWaves * kVBytes;
+  __shared__ __align__(16) unsigned char smem[kWork > kWaves * kOBytes ? kWork : kWaves * kOBytes];
   __shared__ float s_m[kWaves][kCols], s_l[kWaves][kCols];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -175,14 +182,11 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attn_kernel(SharedArgs 
   const int kvh = blockIdx.x % Hkv;
   int u = blockIdx.x / Hkv;
   const int n_prefix = a.col_blocks * a.n_pre;
-  int row_b, lo, hi, slot, b_col, g_col;
-  bool valid;
-  if (u < n_prefix) {
+  const bool prefix = u < n_prefix;
+  int row_b, lo, hi, slot, first_row;  // first_row: of the batch's rows b G + g (prefix), the head (own)
+  if (prefix) {
     const int part = u / a.col_blocks;
-    const int r = (u % a.col_blocks) * kCols + col;
-    b_col = r / G;
-    g_col = r % G;
-    valid = b_col < a.p.B && stream_len(a, min(b_col, a.p.B - 1)) >= P;
+    first_row = (u % a.col_blocks) * kCols;
     row_b = 0;
     lo = part * a.pre_tiles * kTile;
     hi = min(lo + a.pre_tiles * kTile, P);
@@ -191,12 +195,12 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attn_kernel(SharedArgs 
     u -= n_prefix;
     const int part = u % a.n_own;
     u /= a.n_own;
-    g_col = (u % a.own_chunks) * kCols + col;
-    b_col = u / a.own_chunks;
-    valid = g_col < G;
-    const int S = stream_len(a, b_col);
+    first_row = (u % a.own_chunks) * kCols;
+    const int b = u / a.own_chunks;
+    const int S = stream_len(a, b);
     const int first = S < P ? 0 : P;
-    row_b = S < P ? 0 : b_col;
+    row_b = S < P ? 0 : b;
+    u = b;
     // whole tiles, counted from the tile that `first` lies in
     const int t0 = first / kTile, n = (S + kTile - 1) / kTile - t0;
     const int per = (n + a.n_own - 1) / a.n_own;
@@ -204,7 +208,17 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attn_kernel(SharedArgs 
     hi = min(S, (t0 + (part + 1) * per) * kTile);
     slot = a.n_pre + part;
   }
-  if (!valid) b_col = 0, g_col = 0;  // reads an existing row, writes nothing
+  // stream and head (of the kv head's G) of column c; false: there is none
+  auto column = [&](int c, int* b, int* g) {
+    if (prefix) {
+      *b = (first_row + c) / G;
+      *g = (first_row + c) % G;
+      return *b < a.p.B;
+    }
+    *b = u;
+    *g = first_row + c;
+    return *g < G;
+  };
 
   float m = -INFINITY, l = 0.0f;
   f32x16_t o[ND] = {};
@@ -214,53 +228,69 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attn_kernel(SharedArgs 
   Tile<Q8, DH> nxt;
   if (tile < t_end) load_tile(nxt, a, row_b, kvh, tile, last_blk, lane);
 
-  // q as three terms: column `col`, the dims of each k-step and half
-  uint4 q[NS][3];
-  const float* qrow = a.p.q + (static_cast<long>(b_col) * Hq + kvh * G + g_col) * DH;
+  // ---- q as three terms in LDS, rows of columns; columns that there are not hold zeros ----
+  uint16_t* qt = reinterpret_cast<uint16_t*>(smem);
+  if (t_end > 0) {
+    for (int i = tid; i < kCols * (DH / 8); i += 64 * kWaves) {
+      const int c = i / (DH / 8), d = 8 * (i % (DH / 8));
+      int b, g;
+      float x[8] = {};
+      if (column(c, &b, &g)) {
+        const float* row = a.p.q + (static_cast<long>(b) * Hq + kvh * G + g) * DH + d;
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    float x[8];
+        for (int e = 0; e < 8; ++e) x[e] = row[e] * a.scale_log2e;
+      }
+      uint4 t[3];
+      split3(x, t);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = qrow[dim_of<Q8>(s, h) + e];
-    split3(x, q[s]);
+      for (int k = 0; k < 3; ++k)
+        *reinterpret_cast<uint4*>(qt + k * kQTerm + c * kQStride<DH> + d) = t[k];
+    }
   }
-  uint16_t* vt = reinterpret_cast<uint16_t*>(smem + wave * kVBytes);
+  __syncthreads();
+  const uint16_t* qcol = qt + col * kQStride<DH>;
+  uint16_t* vt = reinterpret_cast<uint16_t*>(smem + kQBytes + wave * kVBytes);
 
-  for (; tile < t_end; tile += kWaves) {
-    const Tile<Q8, DH> cur = nxt;
-    if (tile + kWaves < t_end) load_tile(nxt, a, row_b, kvh, tile + kWaves, last_blk, lane);
+  auto work = [&](Tile<Q8, DH>& cur) {
     const int key0 = kTile * tile + 16 * h;  // this lane's 16 keys
     const bool mapped = h ? cur.mapped1 : cur.mapped0;
     const bool whole = cur.mapped0 && cur.mapped1 && kTile * tile >= lo && kTile * (tile + 1) <= hi;
     if constexpr (!Q8) {
       constexpr int LPR = DH / 8, RPI = 64 / LPR;
-      // rows that are not attended go in as zeros: their weights are 0, and 0 * inf is NaN
+      if (!whole) {
+        // rows that are not attended go in as zeros: their weights are 0, and 0 * inf is NaN
 #pragma unroll
-      for (int i = 0; i < DH / 16; ++i) {
-        const int r = RPI * i + lane / LPR, key = kTile * tile + r;
-        const bool in = whole || ((RPI * i < 16 ? cur.mapped0 : cur.mapped1) && key >= lo && key < hi);
-        *reinterpret_cast<uint4*>(vt + r * kVStride<DH> + 8 * (lane % LPR)) =
-            in ? cur.v[i] : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < DH / 16; ++i) {
+          const int key = kTile * tile + RPI * i + lane / LPR;
+          if (!(RPI * i < 16 ? cur.mapped0 : cur.mapped1) || key < lo || key >= hi)
+            cur.v[i] = make_uint4(0, 0, 0, 0);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < DH / 16; ++i)
+        *reinterpret_cast<uint4*>(vt + (RPI * i + lane / LPR) * kVStride<DH> + 8 * (lane % LPR)) =
+            cur.v[i];
     }
     f32x16_t sc = {};
 #pragma unroll
-    for (int k = 2; k >= 0; --k)  // the small terms first
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        uint4 kf;
-        if constexpr (Q8) {
-          const uint4 c = cur.k[s >> 1];
-          kf = (s & 1) ? codes_bf16(c.z, c.w) : codes_bf16(c.x, c.y);
-        } else {
-          kf = cur.k[s];
-        }
-        sc = mfma32(as_bf16x8(kf), as_bf16x8(q[s][k]), sc);
+    for (int s = 0; s < NS; ++s) {
+      uint4 kf;
+      if constexpr (Q8) {
+        const uint4 c = cur.k[s >> 1];
+        kf = (s & 1) ? codes_bf16(c.z, c.w) : codes_bf16(c.x, c.y);
+      } else {
+        kf = cur.k[s];
       }
+#pragma unroll
+      for (int k = 2; k >= 0; --k) {
+        const uint4 qf = *reinterpret_cast<const uint4*>(qcol + k * kQTerm + dim_of<Q8>(s, h));
+        sc = mfma32(as_bf16x8(kf), as_bf16x8(qf), sc);
+      }
+    }
     float x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      x[i] = sc[i] * a.scale_log2e;
+      x[i] = sc[i];
       if constexpr (Q8) x[i] *= reinterpret_cast<const float*>(cur.ks)[i];
     }
     if (!whole) {
@@ -305,7 +335,9 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attn_kernel(SharedArgs 
     }
     if constexpr (!Q8) wave_lds_sync();
 #pragma unroll
-    for (int n = 0; n < ND; ++n)
+    for (int n = 0; n < ND; ++n) {
+      // the codes of one dim block at a time become bf16: all at once are 64 registers
+      if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         uint4 vf;
@@ -322,7 +354,19 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attn_kernel(SharedArgs 
 #pragma unroll
         for (int k = 2; k >= 0; --k) o[n] = mfma32(as_bf16x8(vf), as_bf16x8(wt[s][k]), o[n]);
       }
+    }
     if constexpr (!Q8) wave_lds_sync();  // the tile's buffer is written again
+  };
+  // two tiles' registers in turn: the next one is loaded while one is worked on
+  Tile<Q8, DH> other;
+  while (tile < t_end) {
+    if (tile + kWaves < t_end) load_tile(other, a, row_b, kvh, tile + kWaves, last_blk, lane);
+    work(nxt);
+    tile += kWaves;
+    if (tile >= t_end) break;
+    if (tile + kWaves < t_end) load_tile(nxt, a, row_b, kvh, tile + kWaves, last_blk, lane);
+    work(other);
+    tile += kWaves;
   }
 
   // ---- the waves joined in LDS ----
@@ -333,6 +377,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attn_kernel(SharedArgs 
     s_m[wave][col] = m;
     s_l[wave][col] = l;
   }
+  int unused_b, unused_g;
+  if (column(col, &unused_b, &unused_g))
 #pragma unroll
   for (int n = 0; n < ND; ++n)
 #pragma unroll
@@ -341,21 +387,10 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attn_kernel(SharedArgs 
           make_float4(o[n][4 * r], o[n][4 * r + 1], o[n][4 * r + 2], o[n][4 * r + 3]);
   __syncthreads();
   const float* all = reinterpret_cast<const float*>(smem);
-  const bool prefix = blockIdx.x / Hkv < static_cast<unsigned>(n_prefix);
   for (int i = tid; i < kCols * (DH / 4); i += 64 * kWaves) {
     const int c = i / (DH / 4), d = 4 * (i % (DH / 4));
     int b, g;
-    if (prefix) {
-      const int r = static_cast<int>((blockIdx.x / Hkv) % a.col_blocks) * kCols + c;
-      b = r / G;
-      g = r % G;
-      if (b >= a.p.B) continue;
-    } else {
-      const int v = (blockIdx.x / Hkv - n_prefix) / a.n_own;
-      g = (v % a.own_chunks) * kCols + c;
-      b = v / a.own_chunks;
-      if (g >= G) continue;
-    }
+    if (!column(c, &b, &g)) continue;
     float M = -INFINITY, L = 0.0f;
     float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -393,7 +428,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
   const int lane = threadIdx.x & 63;
   const long row = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= static_cast<long>(a.p.B) * a.p.Hq) return;
-  constexpr int E = DH / 64;
+  constexpr int E = DH / 64, kBatch = 16;
   float M = -INFINITY, L = 0.0f, o[E] = {};
   for (int s0 = 0; s0 < a.slots; s0 += 64) {
     const bool in = s0 + lane < a.slots;
@@ -408,11 +443,20 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] *= c;
     const int n = min(64, a.slots - s0);
-    for (int j = 0; j < n; ++j) {
-      const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
+    for (int j0 = 0; j0 < n; j0 += kBatch) {  // a batch of loads on the way at a time
+      float x[kBatch][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        o[e] = fmaf(wj, a.part_o[(row * a.slots + s0 + j) * DH + 64 * e + lane], o[e]);
+      for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          x[j][e] = a.part_o[(row * a.slots + s0 + min(j0 + j, n - 1)) * DH + 64 * e + lane];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), min(j0 + j, n - 1)));
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (j0 + j < n) o[e] = fmaf(wj, x[j][e], o[e]);
+      }
     }
   }
 #pragma unroll
@@ -442,15 +486,15 @@ int launch_shared_prefix(const KeysProblem& p, const Q8Map& map, hipStream_t str
   a.col_blocks = static_cast<int>((rows + kCols - 1) / kCols);
   a.own_chunks = (a.G + kCols - 1) / kCols;
   const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  // one workgroup per CU for each kind of unit, each of at least one tile per wave
+  // two workgroups per CU for each kind of unit, each of at least one tile per wave
   const long tiles = (p.shared_len + kTile - 1) / kTile;
   const long pre_units = static_cast<long>(a.col_blocks) * p.Hkv;
-  long n_pre = tiles == 0 ? 0 : std::clamp(cus / pre_units, 1L, (tiles + kWaves - 1) / kWaves);
+  long n_pre = tiles == 0 ? 0 : std::clamp(2 * cus / pre_units, 1L, (tiles + kWaves - 1) / kWaves);
   a.pre_tiles = n_pre ? static_cast<int>((tiles + n_pre - 1) / n_pre) : 0;
   a.n_pre = a.pre_tiles ? static_cast<int>((tiles + a.pre_tiles - 1) / a.pre_tiles) : 0;
   const long own = (static_cast<long>(map.capacity) - p.shared_len + kTile - 1) / kTile + 1;
   const long own_units = static_cast<long>(p.B) * p.Hkv * a.own_chunks;
-  a.n_own = static_cast<int>(std::clamp(cus / own_units, 1L, (own + kWaves - 1) / kWaves));
+  a.n_own = static_cast<int>(std::clamp(2 * cus / own_units, 1L, (own + kWaves - 1) / kWaves));
   a.slots = a.n_pre + a.n_own;
   const long grid = pre_units * a.n_pre + own_units * a.n_own;
   if (grid > 0x7fffffffL)
