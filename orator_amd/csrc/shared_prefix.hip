@@ -18,11 +18,14 @@
 //  * a lane has one query column, and scores of 16 consecutive keys: tile row 8 a + 4 h + i is key
 //    16 h + 4 a + i, so lane half h holds block h of the tile and its registers are the B operand
 //    of the second product as they are.
-//  * V^T: bf16 rows through LDS and the transposing read; 8-bit codes lie transposed in memory, a
-//    lane's 16 bytes are its operand.
+//  * bf16 rows are loaded as whole lines and go through LDS: K, then V in its place (V^T by the
+//    transposing read).  8-bit codes go from memory into the operands: K a half line of a row, V as
+//    it lies transposed.
 //  * softmax with a reference that follows the running maximum once it is 8 (log2) behind.
 // The waves of a workgroup take the range's tiles in turn and are joined in LDS; the units'
-// partials of a (stream, head) by a second kernel.
+// partials of a (stream, head) by a second kernel (joined by the last unit to finish, in the same
+// launch, the one that completes a block of columns joins 32 rows alone: B = 64, prefix 4096
+// measured 52 us instead of 41, B = 16 over the 8-bit cache 30 instead of 15).
 #include <algorithm>
 #include <string>
 
@@ -82,6 +85,7 @@ __device__ __forceinline__ void split3(const float (&x)[8], uint4 (&t)[3]) {
 
 // 8 int8 codes (two dwords) as bf16, exact.
 __device__ __forceinline__ uint4 codes_bf16(uint32_t lo, uint32_t hi) {
+  asm volatile("" : "+v"(lo), "+v"(hi));  // converted where it stands, not with the others at once
   float f[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -94,7 +98,7 @@ __device__ __forceinline__ uint4 codes_bf16(uint32_t lo, uint32_t hi) {
 template <bool Q8, int DH>
 struct Tile {
   static constexpr int NK = Q8 ? DH / 32 : DH / 16;  // 16-byte loads of K, and of V
-  uint4 k[NK], v[NK];
+  u32x4_t k[NK], v[NK];  // plain vectors: they have to stay in registers
   float4 ks[Q8 ? 4 : 1], vs[Q8 ? 4 : 1];
   bool mapped0, mapped1;  // the tile's two blocks
 };
@@ -110,10 +114,10 @@ template <bool Q8, int DH>
 __device__ __forceinline__ void load_tile(Tile<Q8, DH>& t, const SharedArgs& a, int row_b, int kvh,
                                           int tile, int last_blk, int lane) {
   const int b0 = min(2 * tile, last_blk), b1 = min(2 * tile + 1, last_blk);
-  const int h = lane >> 5;
-  const bool second = lane & 4;                            // K: the row's block
-  const int at = 4 * ((lane >> 3) & 3) + (lane & 3);       // and its place there
   if constexpr (Q8) {
+    const int h = lane >> 5;
+    const bool second = lane & 4;                       // K: the block of tile row lane & 31
+    const int at = 4 * ((lane >> 3) & 3) + (lane & 3);  // and its place there
     long n0 = a.map.block(row_b, b0, kvh), n1 = a.map.block(row_b, b1, kvh);
     t.mapped0 = n0 >= 0;
     t.mapped1 = n1 >= 0;
@@ -123,9 +127,9 @@ __device__ __forceinline__ void load_tile(Tile<Q8, DH>& t, const SharedArgs& a, 
     const long nv = h ? n1 : n0;
     const int8_t* v = a.p.vq + (nv * DH + (lane & 31)) * kQ8Block;
 #pragma unroll
-    for (int i = 0; i < DH / 32; ++i) t.k[i] = *reinterpret_cast<const uint4*>(k + 32 * i);
+    for (int i = 0; i < DH / 32; ++i) t.k[i] = *reinterpret_cast<const u32x4_t*>(k + 32 * i);
 #pragma unroll
-    for (int i = 0; i < DH / 32; ++i) t.v[i] = *reinterpret_cast<const uint4*>(v + 32 * i * kQ8Block);
+    for (int i = 0; i < DH / 32; ++i) t.v[i] = *reinterpret_cast<const u32x4_t*>(v + 32 * i * kQ8Block);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       t.ks[i] = *reinterpret_cast<const float4*>(a.p.ks + nv * kQ8Block + 4 * i);
@@ -140,23 +144,23 @@ __device__ __forceinline__ void load_tile(Tile<Q8, DH>& t, const SharedArgs& a, 
     // row of the block's first key
     const long r0 = ((static_cast<long>(max(p0, 0)) << bs) + (b0 & msk)) << 4;
     const long r1 = ((static_cast<long>(max(p1, 0)) << bs) + (b1 & msk)) << 4;
-    const uint16_t* k = a.p.kpool + ((second ? r1 : r0) + at) * rs + kvh * DH + 8 * h;
-#pragma unroll
-    for (int i = 0; i < DH / 16; ++i) t.k[i] = *reinterpret_cast<const uint4*>(k + 16 * i);
-    // V rows as they lie: DH / 8 lanes per row, rows in order
+    // rows as they lie, whole lines: DH / 8 lanes per row, rows in order
     constexpr int LPR = DH / 8, RPI = 64 / LPR;  // lanes per row, rows per load
     const uint32_t off = static_cast<uint32_t>(lane / LPR) * static_cast<uint32_t>(rs) + 8 * (lane % LPR);
 #pragma unroll
     for (int i = 0; i < DH / 16; ++i) {
       const int r = RPI * i;  // a load's rows lie in one block (RPI divides 16): a uniform base
-      const uint16_t* v = a.p.vpool + ((r < 16 ? r0 : r1) + (r & 15)) * rs + kvh * DH;
-      t.v[i] = *reinterpret_cast<const uint4*>(v + off);
+      const long at_row = ((r < 16 ? r0 : r1) + (r & 15)) * rs + kvh * DH;
+      t.k[i] = *reinterpret_cast<const u32x4_t*>(a.p.kpool + at_row + off);
+      t.v[i] = *reinterpret_cast<const u32x4_t*>(a.p.vpool + at_row + off);
     }
   }
 }
 
 template <int DH>
 constexpr int kVStride = DH + 16;  // bf16 elements of a V row in LDS
+template <int DH>
+constexpr int kKStride = DH + 8;   // of a K row
 template <int DH>
 constexpr int kQStride = DH + 8;   // and of a q row
 
@@ -181,8 +185,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
   // ---- the unit: its columns, table row and keys [lo, hi) ----
   const int kvh = blockIdx.x % Hkv;
   int u = blockIdx.x / Hkv;
-  const int n_prefix = a.col_blocks * a.n_pre;
-  const bool prefix = u < n_prefix;
+  // the two kinds interleaved: one is bound by the matrix cores, the other by memory
+  const unsigned n_prefix = a.col_blocks * a.n_pre, units = gridDim.x / Hkv;
+  const unsigned before = static_cast<unsigned long>(u) * n_prefix / units;
+  const bool prefix = static_cast<unsigned long>(u + 1) * n_prefix / units > before;
+  u = prefix ? before : u - before;
   int row_b, lo, hi, slot, first_row;  // first_row: of the batch's rows b G + g (prefix), the head (own)
   if (prefix) {
     const int part = u / a.col_blocks;
@@ -192,7 +199,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
     hi = min(lo + a.pre_tiles * kTile, P);
     slot = part;
   } else {
-    u -= n_prefix;
     const int part = u % a.n_own;
     u /= a.n_own;
     first_row = (u % a.own_chunks) * kCols;
@@ -247,45 +253,58 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
         *reinterpret_cast<uint4*>(qt + k * kQTerm + c * kQStride<DH> + d) = t[k];
     }
   }
-  __syncthreads();
+  lds_barrier();  // the first tile's loads stay on the way
   const uint16_t* qcol = qt + col * kQStride<DH>;
   uint16_t* vt = reinterpret_cast<uint16_t*>(smem + kQBytes + wave * kVBytes);
 
-  auto work = [&](Tile<Q8, DH>& cur) {
+  auto work = [&](Tile<Q8, DH>& cur) __attribute__((always_inline)) {
     const int key0 = kTile * tile + 16 * h;  // this lane's 16 keys
     const bool mapped = h ? cur.mapped1 : cur.mapped0;
     const bool whole = cur.mapped0 && cur.mapped1 && kTile * tile >= lo && kTile * (tile + 1) <= hi;
+    constexpr int LPR = DH / 8, RPI = 64 / LPR;
     if constexpr (!Q8) {
-      constexpr int LPR = DH / 8, RPI = 64 / LPR;
+#pragma unroll
+      for (int i = 0; i < DH / 16; ++i)
+        *reinterpret_cast<u32x4_t*>(vt + (RPI * i + lane / LPR) * kKStride<DH> + 8 * (lane % LPR)) =
+            cur.k[i];
       if (!whole) {
         // rows that are not attended go in as zeros: their weights are 0, and 0 * inf is NaN
 #pragma unroll
         for (int i = 0; i < DH / 16; ++i) {
           const int key = kTile * tile + RPI * i + lane / LPR;
           if (!(RPI * i < 16 ? cur.mapped0 : cur.mapped1) || key < lo || key >= hi)
-            cur.v[i] = make_uint4(0, 0, 0, 0);
+            cur.v[i] = u32x4_t{0, 0, 0, 0};
         }
       }
-#pragma unroll
-      for (int i = 0; i < DH / 16; ++i)
-        *reinterpret_cast<uint4*>(vt + (RPI * i + lane / LPR) * kVStride<DH> + 8 * (lane % LPR)) =
-            cur.v[i];
+      wave_lds_sync();
     }
+    // tile row lane & 31: key 16 h + 4 a + i for row 8 a + 4 h + i
+    const uint16_t* krow =
+        vt + (4 * (lane & 4) + 4 * ((lane >> 3) & 3) + (lane & 3)) * kKStride<DH> + 8 * h;
     f32x16_t sc = {};
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       uint4 kf;
       if constexpr (Q8) {
-        const uint4 c = cur.k[s >> 1];
+        // codes become bf16 as they are needed: all at once are too many registers
+        if (s % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+        const u32x4_t c = cur.k[s >> 1];
         kf = (s & 1) ? codes_bf16(c.z, c.w) : codes_bf16(c.x, c.y);
       } else {
-        kf = cur.k[s];
+        kf = *reinterpret_cast<const uint4*>(krow + 16 * s);
       }
 #pragma unroll
       for (int k = 2; k >= 0; --k) {
         const uint4 qf = *reinterpret_cast<const uint4*>(qcol + k * kQTerm + dim_of<Q8>(s, h));
         sc = mfma32(as_bf16x8(kf), as_bf16x8(qf), sc);
       }
+    }
+    if constexpr (!Q8) {  // V takes K's place
+      wave_lds_sync();
+#pragma unroll
+      for (int i = 0; i < DH / 16; ++i)
+        *reinterpret_cast<u32x4_t*>(vt + (RPI * i + lane / LPR) * kVStride<DH> + 8 * (lane % LPR)) =
+            cur.v[i];
     }
     float x[16];
 #pragma unroll
@@ -336,13 +355,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
     if constexpr (!Q8) wave_lds_sync();
 #pragma unroll
     for (int n = 0; n < ND; ++n) {
-      // the codes of one dim block at a time become bf16: all at once are 64 registers
       if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         uint4 vf;
         if constexpr (Q8) {
-          const uint4 c = cur.v[n];
+          const u32x4_t c = cur.v[n];
           vf = s ? codes_bf16(c.z, c.w) : codes_bf16(c.x, c.y);
         } else {
           // keys 16 h + 8 s + 0..3 and + 4..7 of dim 32 n + (lane & 31)
@@ -486,15 +504,16 @@ int launch_shared_prefix(const KeysProblem& p, const Q8Map& map, hipStream_t str
   a.col_blocks = static_cast<int>((rows + kCols - 1) / kCols);
   a.own_chunks = (a.G + kCols - 1) / kCols;
   const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  // two workgroups per CU for each kind of unit, each of at least one tile per wave
+  // Units of at least one tile per wave: up to one workgroup per CU for the prefix, and for the
+  // streams' own keys what is left of the two per CU that run at once.
   const long tiles = (p.shared_len + kTile - 1) / kTile;
   const long pre_units = static_cast<long>(a.col_blocks) * p.Hkv;
-  long n_pre = tiles == 0 ? 0 : std::clamp(2 * cus / pre_units, 1L, (tiles + kWaves - 1) / kWaves);
+  long n_pre = tiles == 0 ? 0 : std::clamp(cus / pre_units, 1L, (tiles + kWaves - 1) / kWaves);
   a.pre_tiles = n_pre ? static_cast<int>((tiles + n_pre - 1) / n_pre) : 0;
   a.n_pre = a.pre_tiles ? static_cast<int>((tiles + a.pre_tiles - 1) / a.pre_tiles) : 0;
   const long own = (static_cast<long>(map.capacity) - p.shared_len + kTile - 1) / kTile + 1;
   const long own_units = static_cast<long>(p.B) * p.Hkv * a.own_chunks;
-  a.n_own = static_cast<int>(std::clamp(2 * cus / own_units, 1L, (own + kWaves - 1) / kWaves));
+  a.n_own = static_cast<int>(std::clamp((2 * cus - pre_units * a.n_pre) / own_units, 1L, (own + kWaves - 1) / kWaves));
   a.slots = a.n_pre + a.n_own;
   const long grid = pre_units * a.n_pre + own_units * a.n_own;
   if (grid > 0x7fffffffL)

@@ -87,6 +87,19 @@ def test_long_prefix(q8):
 
 
 @pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("Hq,Hkv,Dh", [(2, 1, 128), (40, 1, 128), (3, 1, 64)])
+def test_few_heads_and_groups_past_a_block_of_columns(q8, Hq, Hkv, Dh):
+    """One kv head (many splits of the prefix and of a stream's own keys), groups that a block of 32
+    query rows cuts, groups above 32."""
+    check(11, q8, [1500, 1311, 2500, 1300, 1400], 1300, Hq, Hkv, Dh)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_thousands_of_streams(q8):
+    check(12, q8, [33 + b % 3 for b in range(4100)], 32, 1, 1, 64)
+
+
+@pytest.mark.parametrize("q8", [False, True])
 def test_streams_shorter_than_the_prefix(q8):
     """Streams that attend part of the prefix, exactly the prefix, or nothing."""
     check(6, q8, [0, 1, 16, 40, 99, 100, 101, 180, -3], 100)
