@@ -18,9 +18,12 @@
 //    Key (t, i) of a step's tile t is 16 g + 4 t + i for lane group g, so that A and B agree.
 //  So one 64-key step of one wave is 8 + 8 MFMAs of 16 cycles per 4 heads (Dh 128) and about 270
 //  VALU instructions, against 16.5 KB from HBM.
-//  * one workgroup = (split of the keys, kv head, stream), 4 waves that take 64-key steps in turn;
-//    the next step's codes are loaded while the current one is worked on.  Splits are joined by the
-//    last workgroup of a (stream, kv head) to finish.
+//  * one workgroup = (a range of one stream's keys, kv head), 4 waves that take 64-key steps in
+//    turn; the next step's codes are loaded while the current one is worked on.  The streams share
+//    the workgroups of a kv head by their lengths, which every workgroup reads at entry (two
+//    workgroups per CU; streams of 2049 to 4097 keys each cut by the capacity instead left a quarter
+//    of them idle).  A stream's ranges are joined by the last of its workgroups to finish.  Batches
+//    of more streams than that take a workgroup per (stream, kv head).
 #include <algorithm>
 #include <string>
 
@@ -37,13 +40,14 @@ constexpr int kStep = 64;  // keys per wave step
 struct DecodeQ8Args {
   KeysProblem p;
   Q8Map map;
-  int n_splits, split_len;
+  int groups;        // workgroups of a kv head and chunk, shared by the streams; 0: one per stream
   int chunks;        // chunks of 4 NG q heads per kv head
   float scale_log2e;
-  float* part_o;     // [B * Hq][n_splits][Dh]
-  float* part_ml;    // [B * Hq][n_splits][2]
-  unsigned* arrive;  // [B * Hkv * chunks], kCounterStride apart; null: one split
+  float* part_o;     // [Hkv * chunks][groups][4 NG][Dh]
+  float* part_ml;    // [Hkv * chunks][groups][4 NG][2]
+  unsigned* arrive;  // [B * Hkv * chunks], kCounterStride apart
 };
+constexpr int kMaxGroups = 256;
 
 // The four digits of x (|x| <= 2^30), the top one in byte 3.
 __device__ __forceinline__ int digits_of(int x) { return (x + 0x808080) ^ 0x808080; }
@@ -257,29 +261,76 @@ __device__ __forceinline__ void step(RowState<DH, NG>& st, const Q8Step<DH>& kv,
   }
 }
 
+// Keys that stream b attends.
+__device__ __forceinline__ int keys_of(const DecodeQ8Args& a, int b) {
+  const int pos = a.p.pos[b];
+  return pos < 0 ? 0 : min(pos, a.map.capacity - 1) + 1;
+}
+
+// Inclusive sum over the lanes.
+__device__ __forceinline__ int scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+// What a workgroup does: range `part` of `parts` of stream b's S keys; b < 0: nothing.
+struct Share {
+  int b, S, part, parts;
+};
+// Workgroup w of `groups` for up to 64 streams (at most `groups`): stream i gets ceil(steps_i / per)
+// of them, with the smallest per (in rounds of kWaves steps) that `groups` suffice for; each stream
+// at least one.  The same in every wave.
+__device__ __forceinline__ Share share_of(const DecodeQ8Args& a, int w, int lane) {
+  const int S = lane < a.p.B ? keys_of(a, lane) : 0;
+  const int rounds = lane < a.p.B ? max((S + kStep * kWaves - 1) / (kStep * kWaves), 1) : 0;
+  const int total = __builtin_amdgcn_readlane(scan(rounds), 63);
+  int per = (total + a.groups - 1) / a.groups, n, end;
+  for (;; per += 1 + per / 16) {
+    n = (rounds + per - 1) / per;
+    end = scan(n);
+    if (__builtin_amdgcn_readlane(end, 63) <= a.groups) break;  // at the latest at the longest's rounds
+  }
+  const uint64_t mask = __ballot(end > w);
+  if (mask == 0) return {-1, 0, 0, 0};
+  const int b = __builtin_ctzll(mask);
+  const int parts = __builtin_amdgcn_readlane(n, b);
+  return {b, __builtin_amdgcn_readlane(S, b), w - (__builtin_amdgcn_readlane(end, b) - parts), parts};
+}
+
 template <int DH, int NG>
 __global__ __launch_bounds__(64 * kWaves, 2) void decode_q8_kernel(DecodeQ8Args a) {
   constexpr int R = 4 * NG;  // heads of a workgroup
   __shared__ float s_m[kWaves][R], s_l[kWaves][R];
   __shared__ float s_o[kWaves][R][DH];
+  static_assert(R * kMaxGroups <= kWaves * R * DH, "the joining weights take the outputs' place");
   __shared__ int s_last;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int split = blockIdx.x, h = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks;
-  const int b = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks;
   const int G = a.p.Hq / a.p.Hkv;
   const int heads = min(G - chunk * R, R);
+  Share sh;
+  if (a.groups) {
+    sh = share_of(a, blockIdx.x, lane);
+    if (sh.b < 0) return;
+  } else {
+    sh = {static_cast<int>(blockIdx.z), keys_of(a, blockIdx.z), 0, 1};
+  }
+  const int b = sh.b, S = sh.S, part = sh.part, parts = sh.parts;
   const long row0 = static_cast<long>(b) * a.p.Hq + h * G + chunk * R;  // first (stream, q head)
-  const int pos = a.p.pos[b];
-  const int S = pos < 0 ? 0 : min(pos, a.map.capacity - 1) + 1;
-  const int splits = (S + a.split_len - 1) / a.split_len;
-  if (split >= max(splits, 1)) return;
   if (S == 0) {
     for (int i = tid; i < heads * DH; i += 64 * kWaves) a.p.out[row0 * DH + i] = 0.0f;
     return;
   }
   const int last_blk = (S - 1) >> 4;
-  const int s_end = min((split + 1) * (a.split_len / kStep), (S + kStep - 1) / kStep);
-  int s = split * (a.split_len / kStep) + wave;
+  const int steps = (S + kStep - 1) / kStep, per = (steps + parts - 1) / parts;
+  const int s_end = min((part + 1) * per, steps);
+  int s = part * per + wave;
   RowState<DH, NG> st;
   Q8Step<DH> cur, nxt;
   StepBlocks blk{};
@@ -329,51 +380,75 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_q8_kernel(DecodeQ8Args 
       L = fmaf(c, s_l[w][r], L);
       o = fmaf(c, s_o[w][r][d], o);
     }
-    if (splits == 1) {
+    if (parts == 1) {
       a.p.out[row0 * DH + i] = L == 0.0f ? 0.0f : o / L;
     } else {
-      const long ps = (row0 + r) * a.n_splits + split;
-      store_dev(a.part_o + ps * DH + d, o);
+      const long at = (static_cast<long>(blockIdx.y) * a.groups + blockIdx.x) * R + r;
+      store_dev(a.part_o + at * DH + d, o);
       if (d == 0) {
-        store_dev(a.part_ml + 2 * ps, M);
-        store_dev(a.part_ml + 2 * ps + 1, L);
+        store_dev(a.part_ml + 2 * at, M);
+        store_dev(a.part_ml + 2 * at + 1, L);
       }
     }
   }
-  if (splits == 1) return;
-  // ---- the last workgroup of (stream, kv head, chunk) joins the splits ----
+  if (parts == 1) return;
+  // ---- the last workgroup of (stream, kv head, chunk) joins the ranges ----
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
     unsigned* ctr = a.arrive + ((static_cast<long>(b) * a.p.Hkv + h) * a.chunks + chunk) * kCounterStride;
     const unsigned n = __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_last = n + 1 == static_cast<unsigned>(splits);
+    s_last = n + 1 == static_cast<unsigned>(parts);
     if (s_last) __hip_atomic_store(ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (!s_last) return;
-  for (int i = tid; i < heads * DH; i += 64 * kWaves) {
-    const int d = i % DH;
-    const long base = (row0 + i / DH) * a.n_splits;
-    float M = -INFINITY, L = 0.0f, o = 0.0f;
-    for (int j = 0; j < splits; ++j) {
-      const float m = load_dev(a.part_ml + 2 * (base + j));
-      const float l = load_dev(a.part_ml + 2 * (base + j) + 1);
-      const float x = load_dev(a.part_o + (base + j) * DH + d);
-      const float mn = fmaxf(M, m);
-      const float ref = mn == -INFINITY ? 0.0f : mn;
-      const float c0 = fast_exp2(M - ref), c1 = fast_exp2(m - ref);
-      L = fmaf(c1, l, L * c0);
-      o = fmaf(c1, x, o * c0);
-      M = mn;
+  // a head's weights, divided by its sum: one wave a head, a range a lane
+  float* weight = &s_o[0][0][0];  // [R][kMaxGroups]
+  const long first = static_cast<long>(blockIdx.y) * a.groups + blockIdx.x - part;  // the stream's first
+  for (int r = wave; r < heads; r += kWaves) {
+    constexpr int N = kMaxGroups / 64;
+    float m[N], l[N], M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int j = 64 * i + lane;
+      const long at = ((first + min(j, parts - 1)) * R + r) * 2;
+      m[i] = j < parts ? load_dev(a.part_ml + at) : -INFINITY;
+      l[i] = j < parts ? load_dev(a.part_ml + at + 1) : 0.0f;
+      M = fmaxf(M, m[i]);
     }
-    a.p.out[row0 * DH + i] = L == 0.0f ? 0.0f : o / L;
+    M = wave_max(M);
+    const float ref = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int i = 0; i < N; ++i) L = fmaf(fast_exp2(m[i] - ref), l[i], L);
+    L = wave_sum(L);
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (64 * i + lane < parts) weight[r * kMaxGroups + 64 * i + lane] = fast_exp2(m[i] - ref) * inv;
+  }
+  __syncthreads();
+  for (int i = tid; i < heads * DH; i += 64 * kWaves) {
+    const int r = i / DH;
+    const float* from = a.part_o + (first * R + r) * DH + i % DH;
+    constexpr int kBatch = 8;
+    float o = 0.0f;
+    for (int j0 = 0; j0 < parts; j0 += kBatch) {  // a batch of loads on the way at a time
+      float x[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        x[j] = load_dev(from + static_cast<long>(min(j0 + j, parts - 1)) * R * DH);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (j0 + j < parts) o = fmaf(weight[r * kMaxGroups + j0 + j], x[j], o);
+    }
+    a.p.out[row0 * DH + i] = o;
   }
 }
 
 template <int DH, int NG>
 int launch(const DecodeQ8Args& a, hipStream_t stream) {
-  const dim3 grid(a.n_splits, a.p.Hkv * a.chunks, a.p.B);
+  const dim3 grid(a.groups ? a.groups : 1, a.p.Hkv * a.chunks, a.groups ? 1 : a.p.B);
   hipLaunchKernelGGL((decode_q8_kernel<DH, NG>), grid, dim3(64 * kWaves), 0, stream, a);
   return check_launch("decode_q8_kernel");
 }
@@ -388,17 +463,15 @@ int launch_decode_q8(const KeysProblem& p, const Q8Map& map, hipStream_t stream)
   a.map = map;
   a.chunks = (G + 4 * ng - 1) / (4 * ng);
   a.scale_log2e = p.scale * 1.4426950408889634f;
-  const long pairs = static_cast<long>(p.B) * p.Hkv * a.chunks;
-  const long steps = (static_cast<long>(map.capacity) + kStep - 1) / kStep;
-  // two workgroups per CU, splits of at least one step per wave
+  const long heads = static_cast<long>(p.Hkv) * a.chunks;
+  if (heads > 65535) return fail(ORATOR_ERR_UNSUPPORTED, "gqa_decode_q8: too many heads");
   const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  long splits = std::clamp((2 * cus + pairs - 1) / pairs, 1L, (steps + kWaves - 1) / kWaves);
-  if (pairs > kArriveCounters) splits = 1;
-  const long per = (steps + splits - 1) / splits;
-  a.n_splits = static_cast<int>((steps + per - 1) / per);
-  a.split_len = static_cast<int>(per * kStep);
-  if (a.n_splits > 1) {
-    const size_t rows = static_cast<size_t>(p.B) * p.Hq * a.n_splits;
+  // no more than the streams can use: a round of steps each
+  const long rounds = (static_cast<long>(map.capacity) + kStep * kWaves - 1) / (kStep * kWaves);
+  const long groups = std::min(std::min<long>(2 * cus / heads, kMaxGroups), p.B * rounds);
+  if (p.B <= 64 && p.B <= groups && p.B * heads <= kArriveCounters) {
+    a.groups = static_cast<int>(groups);
+    const size_t rows = static_cast<size_t>(heads) * groups * 4 * ng;
     char* ws = static_cast<char*>(workspace_graph(stream, rows * (p.Dh + 2) * sizeof(float), kWsKeys));
     if (!ws) return ORATOR_ERR_HIP;
     a.part_o = reinterpret_cast<float*>(ws);
