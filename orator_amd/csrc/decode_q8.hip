@@ -129,7 +129,7 @@ __device__ __forceinline__ void load_step(Q8Step<DH>& st, const KeysProblem& p, 
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int c = 0; c < DH / 64; ++c) st.k[t][c] = load_nt(k + 4 * t * DH + 64 * c);
+    for (int c = 0; c < DH / 64; ++c) st.k[t][c] = *reinterpret_cast<const uint4*>(k + 4 * t * DH + 64 * c);
 #pragma unroll
   for (int n = 0; n < DH / 16; ++n) st.v[n] = load_nt(v + 256 * n);
   const float* ks = p.ks + bv * kQ8Block + (lane & 3);
@@ -193,10 +193,10 @@ __device__ __forceinline__ void load_q(RowState<DH, NG>& st, const float* q, int
   }
 }
 
-// One step: keys 64 s + 16 (l >> 4) + 4 t + (l & 3) of this lane, those in [first, S) attended.
+// One step: keys 64 s + 16 (l >> 4) + 4 t + (l & 3) of this lane, those before S attended.
 template <int DH, int NG>
-__device__ __forceinline__ void step(RowState<DH, NG>& st, const Q8Step<DH>& kv, int s, int first,
-                                     int S, int lane) {
+__device__ __forceinline__ void step(RowState<DH, NG>& st, const Q8Step<DH>& kv, int s, int S,
+                                     int lane) {
   const bool odd = lane & 1, high = lane & 2;
   const uint32_t sel = byte_sel(3 - (lane & 3));
   const int key0 = kStep * s + 16 * (lane >> 4) + (lane & 3);
@@ -216,7 +216,7 @@ __device__ __forceinline__ void step(RowState<DH, NG>& st, const Q8Step<DH>& kv,
       const float y1 = (odd ? x[3] : x[2]) + dpp<0xB1>(odd ? x[2] : x[3]);
       const float z = (high ? y1 : y0) + dpp<0x4E>(high ? y0 : y1);
       const int key = key0 + 4 * t;
-      const bool in = kv.mapped && key >= first && key < S;
+      const bool in = kv.mapped && key < S;
       sc[t] = in ? z * kv.ks[t] : -INFINITY;
     }
     const float mn = fmaxf(
@@ -228,7 +228,7 @@ __device__ __forceinline__ void step(RowState<DH, NG>& st, const Q8Step<DH>& kv,
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int key = key0 + 4 * t;
-      const bool in = kv.mapped && key >= first && key < S;
+      const bool in = kv.mapped && key < S;
       const float p = fast_exp2(sc[t] - ref);
       w[t] = in ? p * kv.vs[t] : 0.0f;
       // 0 w: a value's scale that is not finite has to show, and digits cannot hold it
@@ -345,14 +345,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_q8_kernel(DecodeQ8Args 
       load_step(nxt, a.p, blk, lane);
       if (s + 2 * kWaves < s_end) blk = step_blocks(a.map, b, h, s + 2 * kWaves, last_blk, lane);
     }
-    step<DH, NG>(st, cur, s, 0, S, lane);
+    step<DH, NG>(st, cur, s, S, lane);
     s += kWaves;
     if (s >= s_end) break;
     if (s + kWaves < s_end) {
       load_step(cur, a.p, blk, lane);
       if (s + 2 * kWaves < s_end) blk = step_blocks(a.map, b, h, s + 2 * kWaves, last_blk, lane);
     }
-    step<DH, NG>(st, nxt, s, 0, S, lane);
+    step<DH, NG>(st, nxt, s, S, lane);
     s += kWaves;
   }
   // ---- the waves' states joined in LDS ----
