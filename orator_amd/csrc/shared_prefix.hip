@@ -103,6 +103,32 @@ struct Tile {
   bool mapped0, mapped1;  // the tile's two blocks
 };
 
+// The rows of a bf16 tile in the pool.
+struct TileRows {
+  long r0, r1;            // of its two blocks' first keys
+  bool mapped0, mapped1;  // (unmapped: rows of page 0, which are masked)
+};
+__device__ __forceinline__ TileRows tile_rows(const SharedArgs& a, int row_b, int tile, int last_blk) {
+  const int b0 = min(2 * tile, last_blk), b1 = min(2 * tile + 1, last_blk);
+  const int p0 = a.map.page(row_b, b0), p1 = a.map.page(row_b, b1);
+  const int bs = a.map.block_shift, msk = (1 << bs) - 1;
+  return {((static_cast<long>(max(p0, 0)) << bs) + (b0 & msk)) << 4,
+          ((static_cast<long>(max(p1, 0)) << bs) + (b1 & msk)) << 4, p0 >= 0, p1 >= 0};
+}
+// A bf16 tile of K or V, rows as they lie, whole lines: DH / 8 lanes per row, rows in order.
+template <int DH>
+__device__ __forceinline__ void load_rows(u32x4_t (&r)[DH / 16], const uint16_t* pool,
+                                          const TileRows& t, long rs, int kvh, int lane) {
+  constexpr int LPR = DH / 8, RPI = 64 / LPR;  // lanes per row, rows per load
+  const uint32_t off = static_cast<uint32_t>(lane / LPR) * static_cast<uint32_t>(rs) + 8 * (lane % LPR);
+#pragma unroll
+  for (int i = 0; i < DH / 16; ++i) {
+    const int row = RPI * i;  // a load's rows lie in one block (RPI divides 16): a uniform base
+    const uint16_t* at = pool + ((row < 16 ? t.r0 : t.r1) + (row & 15)) * rs + kvh * DH;
+    r[i] = *reinterpret_cast<const u32x4_t*>(at + off);
+  }
+}
+
 // The dims of k-step s, lane half h, element e: bf16 K is loaded 8 dims at a time, the 8-bit codes
 // 16 at a time, which serve two k-steps.
 template <bool Q8>
@@ -110,50 +136,30 @@ __device__ __forceinline__ int dim_of(int s, int h) {
   return Q8 ? 32 * (s >> 1) + 16 * h + 8 * (s & 1) : 16 * s + 8 * h;
 }
 
-template <bool Q8, int DH>
-__device__ __forceinline__ void load_tile(Tile<Q8, DH>& t, const SharedArgs& a, int row_b, int kvh,
+// An 8-bit tile.
+template <int DH>
+__device__ __forceinline__ void load_tile(Tile<true, DH>& t, const SharedArgs& a, int row_b, int kvh,
                                           int tile, int last_blk, int lane) {
   const int b0 = min(2 * tile, last_blk), b1 = min(2 * tile + 1, last_blk);
-  if constexpr (Q8) {
-    const int h = lane >> 5;
-    const bool second = lane & 4;                       // K: the block of tile row lane & 31
-    const int at = 4 * ((lane >> 3) & 3) + (lane & 3);  // and its place there
-    long n0 = a.map.block(row_b, b0, kvh), n1 = a.map.block(row_b, b1, kvh);
-    t.mapped0 = n0 >= 0;
-    t.mapped1 = n1 >= 0;
-    n0 = max(n0, 0L);  // unmapped: block 0 is read, its keys are masked
-    n1 = max(n1, 0L);
-    const int8_t* k = a.p.kq + ((second ? n1 : n0) * kQ8Block + at) * DH + 16 * h;
-    const long nv = h ? n1 : n0;
-    const int8_t* v = a.p.vq + (nv * DH + (lane & 31)) * kQ8Block;
+  const int h = lane >> 5;
+  const bool second = lane & 4;                       // K: the block of tile row lane & 31
+  const int at = 4 * ((lane >> 3) & 3) + (lane & 3);  // and its place there
+  long n0 = a.map.block(row_b, b0, kvh), n1 = a.map.block(row_b, b1, kvh);
+  t.mapped0 = n0 >= 0;
+  t.mapped1 = n1 >= 0;
+  n0 = max(n0, 0L);  // unmapped: block 0 is read, its keys are masked
+  n1 = max(n1, 0L);
+  const int8_t* k = a.p.kq + ((second ? n1 : n0) * kQ8Block + at) * DH + 16 * h;
+  const long nv = h ? n1 : n0;
+  const int8_t* v = a.p.vq + (nv * DH + (lane & 31)) * kQ8Block;
 #pragma unroll
-    for (int i = 0; i < DH / 32; ++i) t.k[i] = *reinterpret_cast<const u32x4_t*>(k + 32 * i);
+  for (int i = 0; i < DH / 32; ++i) t.k[i] = *reinterpret_cast<const u32x4_t*>(k + 32 * i);
 #pragma unroll
-    for (int i = 0; i < DH / 32; ++i) t.v[i] = *reinterpret_cast<const u32x4_t*>(v + 32 * i * kQ8Block);
+  for (int i = 0; i < DH / 32; ++i) t.v[i] = *reinterpret_cast<const u32x4_t*>(v + 32 * i * kQ8Block);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      t.ks[i] = *reinterpret_cast<const float4*>(a.p.ks + nv * kQ8Block + 4 * i);
-      t.vs[i] = *reinterpret_cast<const float4*>(a.p.vs + nv * kQ8Block + 4 * i);
-    }
-  } else {
-    const int p0 = a.map.page(row_b, b0), p1 = a.map.page(row_b, b1);
-    t.mapped0 = p0 >= 0;
-    t.mapped1 = p1 >= 0;
-    const int bs = a.map.block_shift, msk = (1 << bs) - 1;
-    const long rs = static_cast<long>(a.p.Hkv) * DH;
-    // row of the block's first key
-    const long r0 = ((static_cast<long>(max(p0, 0)) << bs) + (b0 & msk)) << 4;
-    const long r1 = ((static_cast<long>(max(p1, 0)) << bs) + (b1 & msk)) << 4;
-    // rows as they lie, whole lines: DH / 8 lanes per row, rows in order
-    constexpr int LPR = DH / 8, RPI = 64 / LPR;  // lanes per row, rows per load
-    const uint32_t off = static_cast<uint32_t>(lane / LPR) * static_cast<uint32_t>(rs) + 8 * (lane % LPR);
-#pragma unroll
-    for (int i = 0; i < DH / 16; ++i) {
-      const int r = RPI * i;  // a load's rows lie in one block (RPI divides 16): a uniform base
-      const long at_row = ((r < 16 ? r0 : r1) + (r & 15)) * rs + kvh * DH;
-      t.k[i] = *reinterpret_cast<const u32x4_t*>(a.p.kpool + at_row + off);
-      t.v[i] = *reinterpret_cast<const u32x4_t*>(a.p.vpool + at_row + off);
-    }
+  for (int i = 0; i < 4; ++i) {
+    t.ks[i] = *reinterpret_cast<const float4*>(a.p.ks + nv * kQ8Block + 4 * i);
+    t.vs[i] = *reinterpret_cast<const float4*>(a.p.vs + nv * kQ8Block + 4 * i);
   }
 }
 
@@ -232,7 +238,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
   int tile = lo / kTile + wave;
   const int last_blk = (hi - 1) >> 4;
   Tile<Q8, DH> nxt;
-  if (tile < t_end) load_tile(nxt, a, row_b, kvh, tile, last_blk, lane);
+  const long rs = static_cast<long>(Hkv) * DH;
+  TileRows rows{};  // bf16: of the tile in nxt
+  if (tile < t_end) {
+    if constexpr (Q8) {
+      load_tile(nxt, a, row_b, kvh, tile, last_blk, lane);
+    } else {
+      rows = tile_rows(a, row_b, tile, last_blk);
+      load_rows<DH>(nxt.k, a.p.kpool, rows, rs, kvh, lane);
+      load_rows<DH>(nxt.v, a.p.vpool, rows, rs, kvh, lane);
+    }
+  }
 
   // ---- q as three terms in LDS, rows of columns; columns that there are not hold zeros ----
   uint16_t* qt = reinterpret_cast<uint16_t*>(smem);
@@ -259,8 +275,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
 
   auto work = [&](Tile<Q8, DH>& cur) __attribute__((always_inline)) {
     const int key0 = kTile * tile + 16 * h;  // this lane's 16 keys
-    const bool mapped = h ? cur.mapped1 : cur.mapped0;
-    const bool whole = cur.mapped0 && cur.mapped1 && kTile * tile >= lo && kTile * (tile + 1) <= hi;
+    const bool mapped0 = Q8 ? cur.mapped0 : rows.mapped0, mapped1 = Q8 ? cur.mapped1 : rows.mapped1;
+    const bool mapped = h ? mapped1 : mapped0;
+    const bool whole = mapped0 && mapped1 && kTile * tile >= lo && kTile * (tile + 1) <= hi;
+    const bool more = tile + kWaves < t_end;  // bf16: the next tile takes this one's registers
     constexpr int LPR = DH / 8, RPI = 64 / LPR;
     if constexpr (!Q8) {
 #pragma unroll
@@ -272,9 +290,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
 #pragma unroll
         for (int i = 0; i < DH / 16; ++i) {
           const int key = kTile * tile + RPI * i + lane / LPR;
-          if (!(RPI * i < 16 ? cur.mapped0 : cur.mapped1) || key < lo || key >= hi)
+          if (!(RPI * i < 16 ? mapped0 : mapped1) || key < lo || key >= hi)
             cur.v[i] = u32x4_t{0, 0, 0, 0};
         }
+      }
+      if (more) {
+        rows = tile_rows(a, row_b, tile + kWaves, last_blk);
+        load_rows<DH>(cur.k, a.p.kpool, rows, rs, kvh, lane);
       }
       wave_lds_sync();
     }
@@ -305,6 +327,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
       for (int i = 0; i < DH / 16; ++i)
         *reinterpret_cast<u32x4_t*>(vt + (RPI * i + lane / LPR) * kVStride<DH> + 8 * (lane % LPR)) =
             cur.v[i];
+      if (more) load_rows<DH>(cur.v, a.p.vpool, rows, rs, kvh, lane);
     }
     float x[16];
 #pragma unroll
@@ -375,16 +398,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
     }
     if constexpr (!Q8) wave_lds_sync();  // the tile's buffer is written again
   };
-  // two tiles' registers in turn: the next one is loaded while one is worked on
-  Tile<Q8, DH> other;
-  while (tile < t_end) {
-    if (tile + kWaves < t_end) load_tile(other, a, row_b, kvh, tile + kWaves, last_blk, lane);
-    work(nxt);
-    tile += kWaves;
-    if (tile >= t_end) break;
-    if (tile + kWaves < t_end) load_tile(nxt, a, row_b, kvh, tile + kWaves, last_blk, lane);
-    work(other);
-    tile += kWaves;
+  if constexpr (Q8) {
+    // two tiles' registers in turn: the next one is loaded while one is worked on
+    Tile<Q8, DH> other;
+    while (tile < t_end) {
+      if (tile + kWaves < t_end) load_tile(other, a, row_b, kvh, tile + kWaves, last_blk, lane);
+      work(nxt);
+      tile += kWaves;
+      if (tile >= t_end) break;
+      if (tile + kWaves < t_end) load_tile(nxt, a, row_b, kvh, tile + kWaves, last_blk, lane);
+      work(other);
+      tile += kWaves;
+    }
+  } else {
+    for (; tile < t_end; tile += kWaves) work(nxt);
   }
 
   // ---- the waves joined in LDS ----
