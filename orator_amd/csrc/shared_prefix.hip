@@ -39,6 +39,8 @@ constexpr int kWaves = 4;
 constexpr int kTile = 32;     // keys per wave tile
 constexpr int kCols = 32;     // query columns of a unit
 constexpr float kSlack = 8.0f;
+// instruction kinds of __builtin_amdgcn_sched_group_barrier
+constexpr int kMfma = 0x008, kDsRead = 0x100;
 
 struct SharedArgs {
   KeysProblem p;
@@ -191,11 +193,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
   // ---- the unit: its columns, table row and keys [lo, hi) ----
   const int kvh = blockIdx.x % Hkv;
   int u = blockIdx.x / Hkv;
-  // the two kinds interleaved: one is bound by the matrix cores, the other by memory
-  const unsigned n_prefix = a.col_blocks * a.n_pre, units = gridDim.x / Hkv;
-  const unsigned before = static_cast<unsigned long>(u) * n_prefix / units;
-  const bool prefix = static_cast<unsigned long>(u + 1) * n_prefix / units > before;
-  u = prefix ? before : u - before;
+  // the prefix's units first: they are the longer ones
+  const int n_prefix = a.col_blocks * a.n_pre;
+  const bool prefix = u < n_prefix;
+  if (!prefix) u -= n_prefix;
   int row_b, lo, hi, slot, first_row;  // first_row: of the batch's rows b G + g (prefix), the head (own)
   if (prefix) {
     const int part = u / a.col_blocks;
@@ -321,7 +322,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
         sc = mfma32(as_bf16x8(kf), as_bf16x8(qf), sc);
       }
     }
-    if constexpr (!Q8) {  // V takes K's place
+    if constexpr (!Q8) {
+      // a k-step's operands are read ahead of the products of the one before
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 8, 0);
+#pragma unroll
+      for (int s = 0; s < NS - 2; ++s) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 3, 0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(kMfma, 6, 0);
+      // V takes K's place
       wave_lds_sync();
 #pragma unroll
       for (int i = 0; i < DH / 16; ++i)
