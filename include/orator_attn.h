@@ -235,6 +235,12 @@ int orator_gqa_decode_append_paged(const float* q, const float* k_new, const flo
                                    float* out, int B, int Hq, int Hkv, int Dh, float scale,
                                    void* stream);
 
+/* The operators from here to the decode behind one prefix, and orator_token_logprobs, need no
+ * orator_workspace_reserve: a call that is captured into a graph allocates scratch of its graph's
+ * own, kept until the captured stream is released (orator_stream_destroy), so graphs captured on one
+ * stream may be replayed at the same time.  Eager calls share the scratch of their (device, stream,
+ * host thread). */
+
 /* ------------------------------------------------------------ KV cache in 8 bits ---- */
 /* No counterpart in the reference: a KV cache of one byte per value and one fp32 scale per
  * position and kv head, 0.52 of the bf16 cache's bytes at Dh 128.
@@ -252,8 +258,8 @@ int orator_gqa_decode_append_paged(const float* q, const float* k_new, const flo
  * page_table[b * max_pages + i] names the page of stream b's positions [i * page_size,
  * (i + 1) * page_size).  A contiguous cache is one page of `capacity` positions (capacity a
  * multiple of 16).  kq, vq, ks and vs are 16-byte aligned.  Dh: a multiple of 16, at most 256 (64
- * and 128 run on the kernels built for them, others on generic ones).  Pages named by a negative
- * entry or one >= n_pages are unmapped: they are neither written nor read. */
+ * and 128 run on the kernels built for them, others on generic ones); at most 65535 streams.  Pages
+ * named by a negative entry or one >= n_pages are unmapped: they are neither written nor read. */
 
 /* The rows k, v [Tq][Hkv][Dh] (fp32, row t at t * kv_stride elements, heads contiguous) go to
  * positions *d_pos0 + t.  Rows outside [0, capacity) are not written. */
@@ -262,7 +268,8 @@ int orator_kv_write_q8(const float* k, const float* v, long kv_stride, int8_t* k
                        int capacity, void* stream);
 /* Paged form: stream b's Tq rows (row t at (b * Tq + t) * kv_stride) go to positions d_pos0[b] + t
  * through page-table row b.  Rows outside the table or of unmapped pages are not written; two
- * streams must not write the same page. */
+ * streams must not write the same page.  A stream that has nothing to write in a padded batch
+ * passes d_pos0[b] <= -Tq. */
 int orator_kv_write_q8_paged(const float* k, const float* v, long kv_stride, int8_t* kq, float* ks,
                              int8_t* vq, float* vs, const int* page_table, int max_pages,
                              int page_size, int n_pages, int B, int Tq, int Hkv, int Dh,
@@ -296,7 +303,7 @@ int orator_gqa_decode_q8_paged(const float* q, const int8_t* kq, const float* ks
 /* No counterpart in the reference: orator_gqa_decode_paged for a batch whose first shared_len
  * positions are the same rows for every stream (one prompt for all sessions).  Those keys are read
  * once for the whole batch, through page-table row 0; the keys from shared_len on through each
- * stream's own row (the entries of rows b > 0 for pages wholly inside the prefix are not read).
+ * stream's own row (the entries of rows b > 0 for pages wholly inside the prefix may hold anything).
  * Stream b attends d_pos[b] + 1 keys: only the first of the prefix's where that is fewer than
  * shared_len, none (zeros) where d_pos[b] < 0.  Keys of unmapped pages (negative or >= n_pages)
  * are not attended.  shared_len in [0, max_pages * page_size], page_size a power of two >= 16, any

@@ -1,9 +1,10 @@
 // Decode attention over an 8-bit or bf16 paged cache, with an optional shared prefix, for any head
 // size that is a multiple of 16 (up to 256) and any group, and the entry points of both.
 //
-// One wave per (split of 256 keys, q head, stream): a lane scores one key of 64 with q in LDS, the
+// One wave per (split of the keys, q head, stream): a lane scores one key of 64 with q in LDS, the
 // wave's softmax state is updated once per 64 keys, and for the values each lane owns dims lane,
 // lane + 64, ... .  Splits are joined by their maxima and sums in a second kernel.
+#include <algorithm>
 #include <string>
 
 #include "kv_q8.hpp"
@@ -11,12 +12,13 @@
 namespace orator_hip {
 namespace {
 
-constexpr int kGenSplit = 256;
+constexpr int kGenSplit = 256;      // keys of a split, at least
+constexpr int kGenMaxSplits = 64;   // splits of a stream: what the joining scratch is sized by
 
 struct KeysArgs {
   KeysProblem p;
   Q8Map map;
-  int n_splits;
+  int n_splits, split_len;  // a multiple of 64
   float scale_log2e;
   float* part_o;   // [B * Hq][n_splits][Dh]
   float* part_ml;  // [B * Hq][n_splits][2]
@@ -37,7 +39,9 @@ __global__ __launch_bounds__(64) void keys_generic_kernel(KeysArgs a) {
   const int Dh = a.p.Dh, Hkv = a.p.Hkv, h = hq / (a.p.Hq / Hkv);
   const int S = keys_of(a, b);
   const long bh = static_cast<long>(b) * a.p.Hq + hq;
-  const int j0 = split * kGenSplit, j1 = min(j0 + kGenSplit, S);
+  const long from = static_cast<long>(split) * a.split_len;
+  const int j0 = static_cast<int>(min(from, static_cast<long>(S)));
+  const int j1 = static_cast<int>(min(from + a.split_len, static_cast<long>(S)));
   float m = -INFINITY, l = 0.0f, acc[kQ8MaxDh / 64] = {};
   for (int d = lane; d < Dh; d += 64) sq[d] = a.p.q[bh * Dh + d];
   __syncthreads();
@@ -126,11 +130,13 @@ __global__ __launch_bounds__(256) void keys_merge_kernel(KeysArgs a) {
 }  // namespace
 
 int launch_keys_generic(const KeysProblem& p, const Q8Map& map, hipStream_t stream) {
-  const long splits = (static_cast<long>(map.capacity) + kGenSplit - 1) / kGenSplit;
+  const long cap = map.capacity;
+  const long len = std::max<long>(kGenSplit, ((cap + kGenMaxSplits - 1) / kGenMaxSplits + 63) / 64 * 64);
+  const long splits = (cap + len - 1) / len;
   const size_t rows = static_cast<size_t>(p.B) * p.Hq * splits;
   char* ws = static_cast<char*>(workspace_graph(stream, rows * (p.Dh + 2) * sizeof(float), kWsKeys));
   if (!ws) return ORATOR_ERR_HIP;
-  KeysArgs a{p, map, static_cast<int>(splits), p.scale * 1.4426950408889634f,
+  KeysArgs a{p, map, static_cast<int>(splits), static_cast<int>(len), p.scale * 1.4426950408889634f,
              reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws) + rows * p.Dh};
   const dim3 grid(static_cast<unsigned>(splits), p.Hq, p.B);
   if (p.bf16)

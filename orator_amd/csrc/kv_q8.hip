@@ -427,33 +427,41 @@ extern "C" {
 int orator_kv_write_q8(const float* k, const float* v, long kv_stride, int8_t* kq, float* ks,
                        int8_t* vq, float* vs, int Tq, int Hkv, int Dh, const int* d_pos0,
                        int capacity, void* stream) {
-  return launch_write("kv_write_q8", k, v, kv_stride, kq, ks, vq, vs, nullptr, false, 0, 0, 0, 1,
-                      Tq, Hkv, Dh, d_pos0, capacity, static_cast<hipStream_t>(stream));
+  return guarded([&] {
+    return launch_write("kv_write_q8", k, v, kv_stride, kq, ks, vq, vs, nullptr, false, 0, 0, 0, 1,
+                        Tq, Hkv, Dh, d_pos0, capacity, static_cast<hipStream_t>(stream));
+  });
 }
 
 int orator_kv_write_q8_paged(const float* k, const float* v, long kv_stride, int8_t* kq, float* ks,
                              int8_t* vq, float* vs, const int* page_table, int max_pages,
                              int page_size, int n_pages, int B, int Tq, int Hkv, int Dh,
                              const int* d_pos0, void* stream) {
-  return launch_write("kv_write_q8_paged", k, v, kv_stride, kq, ks, vq, vs, page_table, true,
-                      max_pages, page_size, n_pages, B, Tq, Hkv, Dh, d_pos0, 0,
-                      static_cast<hipStream_t>(stream));
+  return guarded([&] {
+    return launch_write("kv_write_q8_paged", k, v, kv_stride, kq, ks, vq, vs, page_table, true,
+                        max_pages, page_size, n_pages, B, Tq, Hkv, Dh, d_pos0, 0,
+                        static_cast<hipStream_t>(stream));
+  });
 }
 
 int orator_kv_read_q8(const int8_t* kq, const float* ks, const int8_t* vq, const float* vs,
                       void* k, void* v, int out_bf16, int Tq, int Hkv, int Dh, const int* d_pos0,
                       int capacity, void* stream) {
-  return launch_read("kv_read_q8", kq, ks, vq, vs, nullptr, false, 0, 0, 0, k, v, out_bf16, 1, Tq,
-                     Hkv, Dh, d_pos0, capacity, static_cast<hipStream_t>(stream));
+  return guarded([&] {
+    return launch_read("kv_read_q8", kq, ks, vq, vs, nullptr, false, 0, 0, 0, k, v, out_bf16, 1, Tq,
+                       Hkv, Dh, d_pos0, capacity, static_cast<hipStream_t>(stream));
+  });
 }
 
 int orator_kv_read_q8_paged(const int8_t* kq, const float* ks, const int8_t* vq, const float* vs,
                             const int* page_table, int max_pages, int page_size, int n_pages,
                             void* k, void* v, int out_bf16, int B, int Tq, int Hkv, int Dh,
                             const int* d_pos0, void* stream) {
-  return launch_read("kv_read_q8_paged", kq, ks, vq, vs, page_table, true, max_pages, page_size,
-                     n_pages, k, v, out_bf16, B, Tq, Hkv, Dh, d_pos0, 0,
-                     static_cast<hipStream_t>(stream));
+  return guarded([&] {
+    return launch_read("kv_read_q8_paged", kq, ks, vq, vs, page_table, true, max_pages, page_size,
+                       n_pages, k, v, out_bf16, B, Tq, Hkv, Dh, d_pos0, 0,
+                       static_cast<hipStream_t>(stream));
+  });
 }
 
 }  // extern "C"

@@ -214,11 +214,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
     const int first = S < P ? 0 : P;
     row_b = S < P ? 0 : b;
     u = b;
-    // whole tiles, counted from the tile that `first` lies in
+    // whole tiles, counted from the tile that `first` lies in (key numbers past 2^31 in 64 bits)
     const int t0 = first / kTile, n = (S + kTile - 1) / kTile - t0;
-    const int per = (n + a.n_own - 1) / a.n_own;
-    lo = max(first, (t0 + part * per) * kTile);
-    hi = min(S, (t0 + (part + 1) * per) * kTile);
+    const long per = (n + a.n_own - 1) / a.n_own;
+    lo = static_cast<int>(max(static_cast<long>(first), min((t0 + part * per) * kTile, static_cast<long>(S))));
+    hi = static_cast<int>(min((t0 + (part + 1) * per) * kTile, static_cast<long>(S)));
     slot = a.n_pre + part;
   }
   // stream and head (of the kv head's G) of column c; false: there is none

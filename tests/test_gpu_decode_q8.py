@@ -161,3 +161,67 @@ def test_write_then_attend():
                                 B, Hq, Hkv, Dh, 0.09)
         want, tol = qm.attend(q, *c.values64(), table, [at] * B, 0.09, 48)
         close(down(out, q.shape), want, tol)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,Dh", [(64, 2, 1, 64), (65, 2, 1, 64), (130, 8, 2, 128),
+                                         (1, 600, 600, 64), (3, 40, 2, 64)])
+def test_many_streams_and_heads(B, Hq, Hkv, Dh):
+    """Batches that share the workgroups by lengths (64 streams at most) and those that do not; very
+    unequal lengths, empty streams among them."""
+    r = SplitMix64(B + Hq)
+    lens = [(0, 1, 700, 33, 64, 257, 5, 130)[b % 8] for b in range(B)] if B > 1 else [100]
+    max_pages = -(-max(lens) // 32)
+    table, n_pages = qm.table_of(r, B, max_pages)
+    c = qm.Cache(n_pages, 32, Hkv, Dh, rng=r)
+    q = r.normal((B, Hq, Dh), 2.0)
+    pos = [n - 1 for n in lens]
+    want, tol = qm.attend(q, *c.values64(), table, pos, 0.1, max_pages * 32)
+    say("decode q8 many", B, Hq, Hkv, Dh)
+    close(run_paged(q, c, table, n_pages, pos, 0.1), want, tol)
+
+
+def test_table_far_longer_than_the_streams():
+    """A table of 131072 positions, streams of a few: what the capacity sizes is not used up."""
+    B, Hq, Hkv, Dh, ps, max_pages = 3, 4, 2, 64, 16, 8192
+    r = SplitMix64(18)
+    table = np.full((B, max_pages), -1, np.int32)
+    table[:, :20] = np.arange(B * 20, dtype=np.int32).reshape(B, 20)
+    c = qm.Cache(B * 20, ps, Hkv, Dh, rng=r)
+    q = r.normal((B, Hq, Dh))
+    pos = [310, 0, 65]
+    want, tol = qm.attend(q, *c.values64(), table, pos, 0.1, max_pages * ps)
+    say("decode q8 long table")
+    close(run_paged(q, c, table, B * 20, pos, 0.1), want, tol)
+
+
+def test_a_pool_past_32_bits():
+    """Pages whose codes lie more than 2^31 bytes into the pool: written, attended, read back."""
+    import torch
+    Hq, Hkv, Dh, ps, T = 4, 8, 128, 128, 300
+    n_pages = (1 << 31) // (Hkv * ps * Dh) + 8
+    r = SplitMix64(19)
+    gpu = lambda *shape, dtype: torch.empty(*shape, dtype=dtype, device="cuda")  # noqa: E731
+    kq, vq = (gpu(n_pages, Hkv * ps * Dh, dtype=torch.int8) for _ in "kv")
+    ks, vs = (gpu(n_pages, Hkv * ps, dtype=torch.float32) for _ in "kv")
+    table = np.array([[n_pages - 1, 0, n_pages - 3]], np.int32)
+    k, v = r.normal((1, T, Hkv, Dh)), r.normal((1, T, Hkv, Dh))
+    cache = [x.data_ptr() for x in (kq, ks, vq, vs)]
+    paging = (up(table), 3, ps, n_pages)
+    say("decode q8 past 32 bits", n_pages)
+    da.WriteKvCacheQ8Paged(up(k), up(v), Hkv * Dh, *cache, *paging, 1, T, Hkv, Dh,
+                           up(np.zeros(1, np.int32)))
+    c = qm.Cache(3, ps, Hkv, Dh)
+    kc, ksc = qm.quantise(k)
+    vc, vsc = qm.quantise(v)
+    for t in range(T):
+        c.write(t // ps, t % ps, slice(None), kc[0, t], ksc[0, t], vc[0, t], vsc[0, t])
+    q = r.normal((1, Hkv * 2, Dh))
+    out, ko, vo = empty(q.shape, np.float32), empty(k.shape, np.float32), empty(v.shape, np.float32)
+    da.GqaDecodeAttnQ8Paged(up(q), *cache, *paging, up(np.array([T - 1], np.int32)), out, 1, Hkv * 2,
+                            Hkv, Dh, 0.1)
+    da.ReadKvCacheQ8Paged(*cache, *paging, ko, vo, False, 1, T, Hkv, Dh, up(np.zeros(1, np.int32)))
+    want, tol = qm.attend(q, *c.values64(), np.arange(3, dtype=np.int32)[None], [T - 1], 0.1, 3 * ps)
+    close(down(out, q.shape), want, tol)
+    kv, vv = c.values()
+    np.testing.assert_array_equal(down(ko, k.shape)[0], kv.reshape(-1, Hkv, Dh)[:T])
+    np.testing.assert_array_equal(down(vo, v.shape)[0], vv.reshape(-1, Hkv, Dh)[:T])

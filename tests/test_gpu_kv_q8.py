@@ -211,3 +211,40 @@ def test_written_rows_read_back_within_half_a_scale():
         s = np.abs(x).max(-1, keepdims=True).astype(np.float64) / 127
         # the scale's and the product's roundings: each 2^-24 of at most 127 scales
         assert (np.abs(down(buf, x.shape) - x.astype(np.float64)) <= s * (0.5 + 127 * 2 * qm.U)).all()
+
+
+@pytest.mark.parametrize("bf16,off", [(False, 4), (True, 2), (True, 8)])
+def test_read_into_unaligned_outputs(bf16, off):
+    """Outputs at their natural alignment only."""
+    Tq, Hkv, Dh, cap = 37, 2, 128, 64
+    r = SplitMix64(41)
+    c = qm.Cache(1, cap, Hkv, Dh, rng=r)
+    kv, vv = c.values()
+    dt = np.uint16 if bf16 else np.float32
+    n = Tq * Hkv * Dh * np.dtype(dt).itemsize
+    dk, dv = empty((n + 16,), np.uint8), empty((n + 16,), np.uint8)
+    say("read q8 unaligned", bf16, off)
+    da.ReadKvCacheQ8(*upload(c), dk.ptr + off, dv.ptr + off, bf16, Tq, Hkv, Dh,
+                     up(np.array([5], np.int32)), cap)
+    for buf, val in ((dk, kv), (dv, vv)):
+        want = np.ascontiguousarray(val[0, 5:5 + Tq])
+        got = down(buf, (n + 16,), np.uint8)[off:off + n].view(dt).reshape(want.shape)
+        np.testing.assert_array_equal(got, orc.to_bf16(want) if bf16 else want)
+
+
+def test_a_stream_of_a_padded_batch_writes_nothing():
+    B, Tq, Hkv, Dh, ps = 3, 20, 2, 64, 16
+    r = SplitMix64(43)
+    k, v = r.normal((B, Tq, Hkv, Dh)), r.normal((B, Tq, Hkv, Dh))
+    table, n_pages = qm.table_of(r, B, 2)
+    want = qm.Cache(n_pages, ps, Hkv, Dh, fill=3)
+    kc, ks = qm.quantise(k)
+    vc, vs = qm.quantise(v)
+    for t in range(Tq):
+        want.write(table[1, (7 + t) // ps], (7 + t) % ps, slice(None), kc[1, t], ks[1, t], vc[1, t],
+                   vs[1, t])
+    bufs = upload(qm.Cache(n_pages, ps, Hkv, Dh, fill=3))
+    say("write q8 padded")
+    da.WriteKvCacheQ8Paged(up(k), up(v), Hkv * Dh, *bufs, up(table), 2, ps, n_pages, B, Tq, Hkv, Dh,
+                           up(np.array([-Tq, 7, -2147483648], np.int32)))
+    check_cache(bufs, want)

@@ -155,3 +155,45 @@ def test_shared_equals_the_plain_paged_decode():
                           up(np.asarray(pos, np.int32)), out, 4, 16, 8, 128, scale)
     close(got, want, tol)
     close(got, down(out, q.shape), 2 * tol)
+
+
+def test_a_bf16_pool_past_32_bits():
+    """Pages whose rows lie more than 2^32 bytes into the pool."""
+    import torch
+    B, Hq, Hkv, Dh, ps, P = 2, 16, 8, 128, 128, 150
+    n_pages = (1 << 32) // (ps * Hkv * Dh * 2) + 6
+    r = SplitMix64(23)
+    table = np.array([[n_pages - 1, n_pages - 2], [-1, n_pages - 5]], np.int32)
+    small = Bf16Pool(3, ps, Hkv, Dh, r)
+    small.v[2, :P % ps] = small.v[1, :P % ps]  # each stream's copy of the page the prefix ends in
+    small.k[2, :P % ps] = small.k[1, :P % ps]
+    pools = []
+    for x in (small.k, small.v):
+        t = torch.empty(n_pages, ps * Hkv * Dh, dtype=torch.int16, device="cuda")
+        for at, page in ((0, n_pages - 1), (1, n_pages - 2), (2, n_pages - 5)):
+            t[page] = torch.from_numpy(x[at].reshape(-1).view(np.int16)).cuda()
+        pools.append(t)
+    torch.cuda.synchronize()
+    q = r.normal((B, Hq, Dh))
+    pos = [200, 180]
+    want, tol = qm.attend(q, *small.values64(), np.array([[0, 1], [0, 2]], np.int32), pos, 0.09, 256, P)
+    out = up(np.zeros(q.shape, np.float32))
+    say("shared past 32 bits", n_pages)
+    da.GqaDecodeAttnSharedPaged(up(q), pools[0].data_ptr(), pools[1].data_ptr(), up(table), 2, ps,
+                                n_pages, up(np.array(pos, np.int32)), P, out, B, Hq, Hkv, Dh, 0.09)
+    close(down(out, q.shape), want, tol)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_infinities_in_q_reach_their_own_rows_only(q8):
+    q, pool, table, n_pages, pos, scale = case(24, q8, [90, 81, 100], 70, 16, 8, 128, 16)
+    want, tol = qm.attend(q, *pool.values64(), table, pos, scale, table.shape[1] * 16, 70)
+    q = q.copy()
+    q[1, 5, 3] = np.inf
+    q[2, 0, 127] = np.nan
+    say("shared q inf", q8)
+    got = run(q, pool, table, n_pages, pos, 70, scale)
+    hit = np.zeros(q.shape[:2], bool)
+    hit[1, 5] = hit[2, 0] = True
+    assert np.isnan(got[hit]).all()
+    close(got[~hit], want[~hit], tol[~hit])

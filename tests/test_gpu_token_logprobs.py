@@ -188,3 +188,21 @@ def test_the_best_alternative_is_what_argmax_takes():
     asr_ops.TokenLogprobs(dx, n, tok, 1, n, 5, lp, en, ids, top)
     assert down(ids, (1, 5), np.int32)[0, 0] == down(tok, (1,), np.int32)[0] == x.argmax()
     assert down(top, (1, 5))[0, 0] == down(lp, (1,))[0]
+
+
+@pytest.mark.parametrize("rows,n", [(1300, 9000), (5000, 300), (300, 5000)])
+def test_many_rows(rows, n):
+    """Rows that a launch takes in several rounds, and more than one launch takes."""
+    r = SplitMix64(rows)
+    check(r.normal((rows, n), 2.0), (r.uniform(rows) * n).astype(np.int32), 4)
+
+
+def test_a_long_vocabulary_and_few_numbers_left():
+    """A million entries; rows with 3 numbers above -infinity, near the end and far apart."""
+    n = 1000003
+    r = SplitMix64(16)
+    x = np.full((3, n), -np.inf, np.float32)
+    x[0] = r.normal((n,), 3.0)
+    x[1, [5, 700001, n - 1]] = [0.5, 2.0, 1.0]
+    x[2, n - 40:] = np.arange(40)
+    check(x, [77, n - 1, n - 1], 32)
