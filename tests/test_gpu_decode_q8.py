@@ -11,6 +11,7 @@ import q8_model as qm
 from gpu_helpers import down, empty, say, up
 from helpers import SplitMix64
 from orator_amd import decoder_attn as da
+from orator_amd.runtime import DeviceBuffer
 from test_gpu_kv_q8 import upload
 
 pytestmark = pytest.mark.gpu
@@ -196,16 +197,12 @@ def test_table_far_longer_than_the_streams():
 
 def test_a_pool_past_32_bits():
     """Pages whose codes lie more than 2^31 bytes into the pool: written, attended, read back."""
-    import torch
-    Hq, Hkv, Dh, ps, T = 4, 8, 128, 128, 300
+    Hkv, Dh, ps, T = 8, 128, 128, 300
     n_pages = (1 << 31) // (Hkv * ps * Dh) + 8
     r = SplitMix64(19)
-    gpu = lambda *shape, dtype: torch.empty(*shape, dtype=dtype, device="cuda")  # noqa: E731
-    kq, vq = (gpu(n_pages, Hkv * ps * Dh, dtype=torch.int8) for _ in "kv")
-    ks, vs = (gpu(n_pages, Hkv * ps, dtype=torch.float32) for _ in "kv")
+    cache = [DeviceBuffer(n_pages * Hkv * ps * n) for n in (Dh, 4, Dh, 4)]
     table = np.array([[n_pages - 1, 0, n_pages - 3]], np.int32)
     k, v = r.normal((1, T, Hkv, Dh)), r.normal((1, T, Hkv, Dh))
-    cache = [x.data_ptr() for x in (kq, ks, vq, vs)]
     paging = (up(table), 3, ps, n_pages)
     say("decode q8 past 32 bits", n_pages)
     da.WriteKvCacheQ8Paged(up(k), up(v), Hkv * Dh, *cache, *paging, 1, T, Hkv, Dh,

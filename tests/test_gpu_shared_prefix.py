@@ -13,6 +13,7 @@ import q8_model as qm
 from gpu_helpers import down, say, up
 from helpers import SplitMix64
 from orator_amd import decoder_attn as da
+from orator_amd.runtime import DeviceBuffer
 from test_gpu_decode_q8 import close
 from test_gpu_kv_q8 import upload
 
@@ -159,7 +160,6 @@ def test_shared_equals_the_plain_paged_decode():
 
 def test_a_bf16_pool_past_32_bits():
     """Pages whose rows lie more than 2^32 bytes into the pool."""
-    import torch
     B, Hq, Hkv, Dh, ps, P = 2, 16, 8, 128, 128, 150
     n_pages = (1 << 32) // (ps * Hkv * Dh * 2) + 6
     r = SplitMix64(23)
@@ -169,17 +169,16 @@ def test_a_bf16_pool_past_32_bits():
     small.k[2, :P % ps] = small.k[1, :P % ps]
     pools = []
     for x in (small.k, small.v):
-        t = torch.empty(n_pages, ps * Hkv * Dh, dtype=torch.int16, device="cuda")
+        pool = DeviceBuffer(n_pages * x[0].nbytes)
         for at, page in ((0, n_pages - 1), (1, n_pages - 2), (2, n_pages - 5)):
-            t[page] = torch.from_numpy(x[at].reshape(-1).view(np.int16)).cuda()
-        pools.append(t)
-    torch.cuda.synchronize()
+            pool.upload(x[at], page * x[0].nbytes)
+        pools.append(pool)
     q = r.normal((B, Hq, Dh))
     pos = [200, 180]
     want, tol = qm.attend(q, *small.values64(), np.array([[0, 1], [0, 2]], np.int32), pos, 0.09, 256, P)
     out = up(np.zeros(q.shape, np.float32))
     say("shared past 32 bits", n_pages)
-    da.GqaDecodeAttnSharedPaged(up(q), pools[0].data_ptr(), pools[1].data_ptr(), up(table), 2, ps,
+    da.GqaDecodeAttnSharedPaged(up(q), *pools, up(table), 2, ps,
                                 n_pages, up(np.array(pos, np.int32)), P, out, B, Hq, Hkv, Dh, 0.09)
     close(down(out, q.shape), want, tol)
 
