@@ -49,7 +49,7 @@ struct LogprobArgs {
   float* entropy;
   int* top_ids;
   float* top_logprobs;
-  int parts, chunks, chunk_len;  // chunks of chunk_len entries (a multiple of 4) per part
+  int parts, chunks;  // chunks of a part (the row's last part may have fewer)
   float* stats;      // [rows][parts][4]: m, S, T
   u64* best;         // [rows][parts][top_k], descending; 0: none
   unsigned* arrive;  // [rows], kCounterStride apart; null: one part
@@ -128,21 +128,22 @@ __device__ __forceinline__ void rank_into(u64* best, const u64* list, int n, int
 
 typedef float Chunk[kVec][4];
 
-// Chunk entries (i * kThreads + tid) * 4 + j of n, as loaded: a group of four that does not lie in
-// the chunk holds its last four entries (chunks of fewer than 4: none), which finish_chunk puts right
-// once they are there.  No branch stands between the loads.
-__device__ __forceinline__ void load_chunk(Chunk& v, const float* x, int n, int tid) {
+// Entries c0 + (i * kThreads + tid) * 4 + j of a part's n, as loaded: a group of four that does not
+// lie in the part holds its last four entries (parts of fewer than 4: none), which finish_chunk puts
+// right once they are there.  No branch stands between the loads, and a chunk behind the part's end
+// reads that one line.
+__device__ __forceinline__ void load_chunk(Chunk& v, const float* x, int c0, int n, int tid) {
   if (n < 4) return;  // uniform
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
-    const Vec4 r = load4(x + min((i * kThreads + tid) * 4, n - 4));
+    const Vec4 r = load4(x + min(c0 + (i * kThreads + tid) * 4, n - 4));
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[i][j] = r.v[j];
   }
 }
-// Entries behind the chunk's end become -infinity.
-__device__ __forceinline__ void finish_chunk(Chunk& v, const float* x, int n, int tid) {
-  if (n == kChunk) return;  // uniform
+// Entries behind the part's end become -infinity.
+__device__ __forceinline__ void finish_chunk(Chunk& v, const float* x, int c0, int n, int tid) {
+  if (n - c0 >= kChunk) return;  // uniform
   if (n < 4) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
@@ -152,8 +153,8 @@ __device__ __forceinline__ void finish_chunk(Chunk& v, const float* x, int n, in
   }
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
-    if ((i + 1) * kThreads * 4 <= n) continue;  // uniform
-    const int past = (i * kThreads + tid) * 4 - (n - 4);  // entries that the load came too early
+    if (c0 + (i + 1) * kThreads * 4 <= n) continue;  // uniform
+    const int past = c0 + (i * kThreads + tid) * 4 - (n - 4);  // entries that the load came too early
     if (past > 0) {
       v[i][0] = past == 1 ? v[i][1] : past == 2 ? v[i][2] : past == 3 ? v[i][3] : -INFINITY;
       v[i][1] = past == 1 ? v[i][2] : past == 2 ? v[i][3] : -INFINITY;
@@ -188,6 +189,8 @@ struct Sums {
 // A wave's list of entries that may be among its k best.
 struct List {
   u64* at;              // kList in LDS
+  float* bounds;        // the waves' `reach`, in LDS: each writes its own, all read the largest
+  int wave = 0;
   int n = 0;            // uniform
   float thr = -FLT_MAX; // entries below are not listed (NaN: none is)
   float reach = -INFINITY;  // k listed entries reach this
@@ -200,6 +203,11 @@ struct List {
                                                    __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
     if (in) at[slot] = key;
     n += __popcll(mask);
+  }
+
+  __device__ __forceinline__ void publish(float r) {
+    reach = fmaxf(reach, r);
+    __hip_atomic_store(bounds + wave, reach, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   }
 
   // The list cut to its k best (it has at least k); later entries have to be above the last.
@@ -221,8 +229,8 @@ struct List {
       if (64 * i + lane < n && rank[i] < k) at[rank[i]] = mine[i];
     wave_lds_sync();
     n = k;
-    reach = value_of(static_cast<uint32_t>(at[k - 1] >> 32));
-    thr = above(reach);
+    publish(value_of(static_cast<uint32_t>(at[k - 1] >> 32)));
+    thr = fmaxf(thr, above(reach));
   }
 
   // The chunk's entries, their ids from id0 on, all higher than those listed.
@@ -230,6 +238,13 @@ struct List {
   __device__ __forceinline__ void take(const Chunk& v, const float (&m4)[kVec], float chunk_max,
                                        int id0, int k, int tid, int lane) {
     lane_max = fmaxf(lane_max, chunk_max);
+    // k entries of the part reach any wave's bound: what is below is not among the part's best
+    // (bounds only grow, so one that is read late costs entries, never loses one)
+    float part = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWavesN; ++w)
+      part = fmaxf(part, __hip_atomic_load(bounds + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+    thr = fmaxf(thr, part);
     const int lanes = __popcll(__ballot(chunk_max >= thr));
     if (lanes == 0) return;
     if (lanes > kFew) {
@@ -244,7 +259,7 @@ struct List {
       if (bound > order_of(-INFINITY)) {
         const float b = value_of(bound);
         // k of the wave's entries so far reach b, and those that do are listed or in this chunk
-        if (b > reach) reach = b;
+        if (b > reach) publish(b);
         if (b > thr) thr = b;
       }
     }
@@ -308,25 +323,27 @@ __global__ __launch_bounds__(kThreads, 5) void token_logprobs_kernel(LogprobArgs
   const int row = blockIdx.x / a.parts;
   const float* x = a.x + row * a.row_stride;
   const int k = a.top_k;
-  const long base = static_cast<long>(part) * a.chunks * a.chunk_len;
+  const long base = static_cast<long>(part) * a.chunks * kChunk;
   x += base;
-  // the part's entries (none for a part behind the row's end)
-  const int entries = static_cast<int>(
-      max(0L, min(static_cast<long>(a.chunks) * a.chunk_len, a.vocab - base)));
+  const int entries = static_cast<int>(min(static_cast<long>(a.chunks) * kChunk, a.vocab - base));
   Sums sum;
   List list;
   list.at = s_list[wave];
+  list.bounds = s_reach;
+  list.wave = wave;
+  if (tid < kWavesN) s_reach[tid] = -INFINITY;
   Chunk nxt = {};
-  load_chunk(nxt, x, min(a.chunk_len, entries), tid);
-  for (int c0 = 0; c0 < entries; c0 += a.chunk_len) {
-    const int n = min(a.chunk_len, entries - c0);
+  load_chunk(nxt, x, 0, entries, tid);
+  lds_barrier();
+  for (long c = 0; c < entries; c += kChunk) {
+    const int c0 = static_cast<int>(c);
     Chunk v;
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[i][j] = nxt[i][j];
-    load_chunk(nxt, x + c0 + a.chunk_len, min(a.chunk_len, entries - c0 - a.chunk_len), tid);
-    finish_chunk(v, x + c0, n, tid);
+    load_chunk(nxt, x, min(c0, 0x7fffffff - 2 * kChunk) + kChunk, entries, tid);
+    finish_chunk(v, x, c0, entries, tid);
     float m4[kVec], mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
@@ -350,7 +367,6 @@ __global__ __launch_bounds__(kThreads, 5) void token_logprobs_kernel(LogprobArgs
   sum.T = wave_sum(sum.T);
   if (lane == 0) {
     s_sums[wave][0] = sum.m, s_sums[wave][1] = sum.S, s_sums[wave][2] = sum.T;
-    s_reach[wave] = list.reach;
     s_len[wave] = list.n;
   }
   if (tid == 0) s_n = 0;
@@ -525,8 +541,6 @@ int token_logprobs(LogprobArgs a, int rows, hipStream_t stream) {
   }
   a.chunks = static_cast<int>((chunks + parts - 1) / parts);
   a.parts = static_cast<int>((chunks + a.chunks - 1) / a.chunks);
-  const long all = static_cast<long>(a.chunks) * a.parts;
-  a.chunk_len = static_cast<int>(((a.vocab + all - 1) / all + 3) / 4 * 4);
   const size_t per_row = static_cast<size_t>(a.parts) * (4 * sizeof(float) + a.top_k * sizeof(u64));
   const int slab = static_cast<int>(
       std::clamp<size_t>(kSlabBytes / per_row, 1, static_cast<size_t>(std::min(rows, kArriveCounters))));
