@@ -24,6 +24,9 @@
 //    workgroups per CU; streams of 2049 to 4097 keys each cut by the capacity instead left a quarter
 //    of them idle).  A stream's ranges are joined by the last of its workgroups to finish.  Batches
 //    of more streams than that take a workgroup per (stream, kv head).
+//  Measured, 16 q / 8 kv heads of 128: 16 streams of 2049 to 4097 keys 24.4 us a call (106 MB, 4.35
+//  TB/s; B = 64 of 4096 keys 98 us, 5.65 TB/s, where a chain of ~6 us weighs less), one stream of
+//  1301 keys 8.0 us, of 16384 keys 16.8 us.
 #include <algorithm>
 #include <string>
 

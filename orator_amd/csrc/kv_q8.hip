@@ -124,8 +124,9 @@ __device__ __forceinline__ BlockItem block_item(const Q8Map& map, const int* pos
     w.block = map.block(w.b, static_cast<int>(blk), w.h);
   return w;
 }
-// Prompts, Dh 64 and 128: one wave per block of 16 positions, head, and K or V.  Memory-bound (5 Dh
-// + 4 bytes per row and head, K and V apart).  K: lanes across a row, 4 dims each, codes stored a
+// Prompts, Dh 64 and 128: one wave per block of 16 positions, head, and K or V.  Bound by VALU work
+// beside the memory (5 Dh + 4 bytes per row and head, K and V apart): 2048 rows of 8 heads of 128 in 9.7
+// us, 2.2 TB/s, with two waves per SIMD.  K: lanes across a row, 4 dims each, codes stored a
 // dword a lane.  V: a lane has Dh / 64 dims of all 16 rows, so that its codes are 16 whole bytes of
 // the transposed block each; a block that the call covers in part is stored byte by byte.
 template <int DH>
@@ -201,7 +202,8 @@ __global__ __launch_bounds__(256) void kv_write_q8_block_kernel(WriteArgs a, int
   if (w.is_v && lane >= w.r0 && lane < w.r1) a.vs[w.block * kQ8Block + lane] = my_scale;
 }
 
-// Single rows, and any Dh: one wave per (token, head, K or V), lane l holds dims 4 l .. 4 l + 3.
+// Few rows, and any Dh: one wave per (token, head, K or V), lane l holds dims 4 l .. 4 l + 3.  A chain
+// of three memory round trips (position, page, row): 16 streams' single rows of 8 heads in 3.3 us.
 __global__ __launch_bounds__(256) void kv_write_q8_kernel(WriteArgs a) {
   const int lane = threadIdx.x & 63;
   const unsigned item = wave_item(), Hkv = a.map.Hkv;
@@ -257,7 +259,8 @@ __device__ __forceinline__ T value_as(float x) {
 }
 
 // Dh 64 and 128: one wave per block of 16 positions, head, and K or V, as the write's block kernel;
-// memory-bound, every load and store a whole line a row.
+// memory-bound, every load and store a whole line a row: 16 x 4096 rows of 8 heads of 128 into fp32 in
+// 115 us, 5.9 TB/s (a wave per row: 476).
 template <int DH, typename T>
 __global__ __launch_bounds__(256) void kv_read_q8_block_kernel(ReadArgs a, int blocks) {
   const int lane = threadIdx.x & 63;
@@ -315,7 +318,7 @@ __global__ __launch_bounds__(256) void kv_read_q8_block_kernel(ReadArgs a, int b
   }
 }
 
-// Any Dh: one wave per (token, head, K or V), as the write.
+// Few rows, and any Dh: one wave per (token, head, K or V), as the write.
 __global__ __launch_bounds__(256) void kv_read_q8_kernel(ReadArgs a) {
   const int lane = threadIdx.x & 63;
   const unsigned item = wave_item(), Hkv = a.map.Hkv;
@@ -344,8 +347,15 @@ __global__ __launch_bounds__(256) void kv_read_q8_kernel(ReadArgs a) {
   }
 }
 
-// Calls of this many rows up take the block kernels.
-constexpr int kBlockRows = 8;
+// Whether a call takes the block kernels: rows that fill their blocks (8 of 16 at least), and more
+// of them than the chip holds waves of the row kernels, one per row, head, and K or V, at once (8 per
+// SIMD; below that the row kernels' shorter chains win).  8 heads of 128, us, row / block kernel:
+// writes of 16 x 16 rows 4.8 / 7.1, 16 x 32 7.0 / 7.3, 16 x 64 10.4 / 8.2, 1 x 64 3.5 / 6.1, 1 x 2048
+// 22.3 / 9.7; reads of 16 x 16 rows 3.9 / 4.5, 16 x 32 5.2 / 5.1, 16 x 64 7.7 / 5.2.
+bool by_blocks(int B, int Tq, int Hkv, int Dh) {
+  const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
+  return (Dh == 64 || Dh == 128) && Tq >= 8 && 2L * B * Tq * Hkv > 32 * cus;
+}
 // Blocks that Tq rows touch at most, from wherever they begin.
 int most_blocks(int Tq) { return static_cast<int>((static_cast<long>(Tq) + 14) / kQ8Block + 1); }
 
@@ -371,7 +381,7 @@ int launch_write(const char* what, const float* k, const float* v, long kv_strid
   if (kv_stride < static_cast<long>(Hkv) * Dh)
     return fail(ORATOR_ERR_INVALID, std::string(what) + ": kv_stride below Hkv * Dh");
   dim3 grid;
-  if ((Dh == 64 || Dh == 128) && Tq >= kBlockRows) {
+  if (by_blocks(B, Tq, Hkv, Dh)) {
     const int blocks = most_blocks(Tq);
     if (int rc = grid_of(2L * blocks * Hkv, B, &grid, what)) return rc;
     if (Dh == 128)
@@ -400,7 +410,7 @@ int launch_read(const char* what, const int8_t* kq, const float* ks, const int8_
     return rc;
   dim3 grid;
   // vector stores: outputs that are 16-byte aligned
-  if ((Dh == 64 || Dh == 128) && Tq >= kBlockRows && aligned_to(k, 16) && aligned_to(v, 16)) {
+  if (by_blocks(B, Tq, Hkv, Dh) && aligned_to(k, 16) && aligned_to(v, 16)) {
     const int blocks = most_blocks(Tq);
     if (int rc = grid_of(2L * blocks * Hkv, B, &grid, what)) return rc;
     auto launch = [&](auto kernel) {

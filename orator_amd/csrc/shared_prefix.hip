@@ -26,6 +26,11 @@
 // partials of a (stream, head) by a second kernel (joined by the last unit to finish, in the same
 // launch, the one that completes a block of columns joins 32 rows alone: B = 64, prefix 4096
 // measured 52 us instead of 41, B = 16 over the 8-bit cache 30 instead of 15).
+//
+// Measured, 16 q / 8 kv heads of 128, both launches: 64 streams behind 4096 keys with 1 to 512 of their
+// own, bf16, 37.9 us (85 MB: 16.5 us at a copy's rate); 16 behind 2048, 8-bit, 14.6 us; 6 behind 503,
+// bf16, 11.1 us.  A tile is 48 MFMAs (0.7 us) and some 430 VALU instructions; two waves per SIMD
+// overlap them to 1.3 us a tile, and a workgroup's start and end cost 7 us.
 #include <algorithm>
 #include <string>
 

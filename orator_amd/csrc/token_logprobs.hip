@@ -11,10 +11,13 @@
 //
 // Best entries: a wave keeps a list in LDS of entries that may be among the k best of its own.  The
 // k-th largest of the 64 lanes' running maxima is a bound that k entries reach, so entries below it
-// are left out (1024 entries of a wave add some 24 at first, then ever fewer).  A chunk with too many (ties
-// in masses) gives its k best one after the other instead; a full list is cut to its k best.  What
+// are left out (1024 entries of a wave add some 24 at first, then ever fewer).  A chunk with too many
+// (ties in masses) gives its k best one after the other instead; a full list is cut to its k best.  What
 // the waves listed is ranked by counting, per part and then per row.  Entries of -infinity and NaN
 // are never listed: a row with fewer than k others is searched for them at the end.
+//
+// Measured, 151936 entries: 257 rows with 20 alternatives 42 us (3.7 TB/s, VALU issue at 65 %; without
+// alternatives 33), one row with 5 9.4 us.
 #include <float.h>
 
 #include <algorithm>

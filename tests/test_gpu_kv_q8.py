@@ -248,3 +248,37 @@ def test_a_stream_of_a_padded_batch_writes_nothing():
     da.WriteKvCacheQ8Paged(up(k), up(v), Hkv * Dh, *bufs, up(table), 2, ps, n_pages, B, Tq, Hkv, Dh,
                            up(np.array([-Tq, 7, -2147483648], np.int32)))
     check_cache(bufs, want)
+
+
+@pytest.mark.parametrize("B,Tq,Hkv,Dh", [(9, 70, 8, 128), (9, 71, 8, 64), (40, 9, 16, 128), (3, 2000, 1, 64)])
+def test_calls_on_both_sides_of_the_block_kernels(B, Tq, Hkv, Dh):
+    """Large calls from odd positions, and the same rows written one stream at a time."""
+    r = SplitMix64(Tq)
+    ps, max_pages = 32, -(-(Tq + 40) // 32)
+    table, n_pages = qm.table_of(r, B, max_pages)
+    pos = np.array([(7 * b) % 33 for b in range(B)], np.int32)
+    k, v = r.normal((B, Tq, Hkv, Dh)), r.normal((B, Tq, Hkv, Dh))
+    bufs, dt = upload(qm.Cache(n_pages, ps, Hkv, Dh, fill=2)), up(table)
+    say("write q8 large", B, Tq, Hkv, Dh)
+    da.WriteKvCacheQ8Paged(up(k), up(v), Hkv * Dh, *bufs, dt, max_pages, ps, n_pages, B, Tq, Hkv, Dh,
+                           up(pos))
+    other = upload(qm.Cache(n_pages, ps, Hkv, Dh, fill=2))
+    for b in range(B):
+        for t in range(0, Tq, 250):
+            n = min(250, Tq - t)
+            da.WriteKvCacheQ8Paged(up(k[b, t:t + n]), up(v[b, t:t + n]), Hkv * Dh, *other,
+                                   up(table[b]), max_pages, ps, n_pages, 1, n, Hkv, Dh,
+                                   up(pos[b:b + 1] + t))
+    want = qm.Cache(n_pages, ps, Hkv, Dh)
+    arrays = (want.kq, want.ks, want.vq, want.vs)
+    for x, y, w in zip(bufs, other, arrays):
+        np.testing.assert_array_equal(down(x, w.shape, w.dtype), down(y, w.shape, w.dtype))
+    kc, ks = qm.quantise(k[B - 1])
+    page, row = table[B - 1][(pos[B - 1] + np.arange(Tq)) // ps], (pos[B - 1] + np.arange(Tq)) % ps
+    np.testing.assert_array_equal(down(bufs[0], want.kq.shape, np.int8)[page, :, row], kc)
+    np.testing.assert_array_equal(down(bufs[1], want.ks.shape)[page, :, row], ks)
+    dk, dv = empty(k.shape, np.float32), empty(v.shape, np.float32)
+    da.ReadKvCacheQ8Paged(*bufs, dt, max_pages, ps, n_pages, dk, dv, False, B, Tq, Hkv, Dh, up(pos))
+    for x, buf in ((k, dk), (v, dv)):
+        c, s = qm.quantise(x)
+        np.testing.assert_array_equal(down(buf, x.shape), c.astype(np.float32) * s[..., None])
