@@ -207,8 +207,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
     const int part = u / a.col_blocks;
     first_row = (u % a.col_blocks) * kCols;
     row_b = 0;
-    lo = part * a.pre_tiles * kTile;
-    hi = min(lo + a.pre_tiles * kTile, P);
+    // (in 64 bits: the last range's end may pass 2^31)
+    const long from = static_cast<long>(part) * a.pre_tiles * kTile;
+    lo = static_cast<int>(min(from, static_cast<long>(P)));
+    hi = static_cast<int>(min(from + static_cast<long>(a.pre_tiles) * kTile, static_cast<long>(P)));
     slot = part;
   } else {
     const int part = u % a.n_own;
@@ -558,7 +560,7 @@ int launch_shared_prefix(const KeysProblem& p, const Q8Map& map, hipStream_t str
   a.n_own = static_cast<int>(std::clamp((2 * cus - pre_units * a.n_pre) / own_units, 1L, (own + kWaves - 1) / kWaves));
   a.slots = a.n_pre + a.n_own;
   const long grid = pre_units * a.n_pre + own_units * a.n_own;
-  if (grid > 0x7fffffffL)
+  if (grid > kMaxGroups256)
     return fail(ORATOR_ERR_UNSUPPORTED, "gqa_decode_shared: too many streams and heads");
   const size_t parts = static_cast<size_t>(p.B) * p.Hq * a.slots;
   char* ws = static_cast<char*>(workspace_graph(stream, parts * (p.Dh + 2) * sizeof(float), kWsKeys));

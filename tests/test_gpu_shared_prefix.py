@@ -196,3 +196,22 @@ def test_infinities_in_q_reach_their_own_rows_only(q8):
     hit[1, 5] = hit[2, 0] = True
     assert np.isnan(got[hit]).all()
     close(got[~hit], want[~hit], tol[~hit])
+
+
+@pytest.mark.parametrize("q8,P", [(False, 1696), (True, 1696), (True, 0)])
+def test_positions_up_to_the_largest(q8, P):
+    """A table of 2^31 positions, of which the first page and the last are mapped: 1024 keys, and
+    those of the last page that an int holds (768); the prefix ends in that page, or there is none."""
+    ps, Hkv, Dh = 1024, 1, 64
+    n = (1 << 31) // ps
+    r = SplitMix64(31)
+    pool = qm.Cache(3, ps, Hkv, Dh, rng=r) if q8 else Bf16Pool(3, ps, Hkv, Dh, r)
+    q = r.normal((2, 2, Dh), 2.0)
+    small = np.array([[0, 1], [0, 2]], np.int32)
+    table = np.full((2, n), -1, np.int32)
+    table[:, 0], table[:, -1] = small[:, 0], small[:, 1]
+    far = (n - 2) * ps  # positions of the last page, less those of a table of two
+    want, tol = qm.attend(q, *pool.values64(), small, [1791, 1750], 0.125, 1792, P)
+    pos = [0x7fffffff, 1750 + far]
+    say("largest positions", q8, P)
+    close(run(q, pool, table, 3, pos, P + far if P else 0, 0.125), want, tol)
