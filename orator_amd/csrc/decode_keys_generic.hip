@@ -164,8 +164,8 @@ int decode_keys(const char* what, const KeysProblem& p, bool paged, hipStream_t 
     return rc;
   }
   if (p.Hq % p.Hkv) return fail(ORATOR_ERR_INVALID, who + ": Hq must be a multiple of Hkv");
-  if (p.B > 65535 || p.Hq > 65535 || static_cast<long>(p.B) * p.Hq > 0x7fffffffL)
-    return fail(ORATOR_ERR_UNSUPPORTED, who + ": at most 65535 streams and q heads");
+  if (p.B > 65535 || p.Hq > 65535 || static_cast<long>(p.B) * p.Hq > kMaxGroups256)
+    return fail(ORATOR_ERR_UNSUPPORTED, who + ": too many streams or q heads");
   Q8Map map;
   if (int rc = q8_map(&map, what, p.page_table, paged, p.max_pages, p.page_size, p.n_pages, p.Hkv,
                       p.Dh, p.capacity))

@@ -361,7 +361,7 @@ int most_blocks(int Tq) { return static_cast<int>((static_cast<long>(Tq) + 14) /
 
 // Grid of B streams of `waves` waves each, 4 to a workgroup.
 int grid_of(long waves, int B, dim3* grid, const char* what) {
-  if (waves > 0x7fffffffL || B > 65535)
+  if ((waves + 3) / 4 > kMaxGroups256 || B > 65535)
     return fail(ORATOR_ERR_UNSUPPORTED, std::string(what) + ": too many rows, or over 65535 streams");
   *grid = dim3(static_cast<unsigned>((waves + 3) / 4), B);
   return ORATOR_OK;

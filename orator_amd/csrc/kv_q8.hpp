@@ -47,6 +47,9 @@ inline bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintpt
 // Largest capacity a launch takes: positions and their successors stay ints.
 constexpr long kQ8MaxCapacity = 0x7fffff00L;
 
+// Workgroups of 256 threads in one dimension of a grid, which holds fewer than 2^32 threads.
+constexpr long kMaxGroups256 = (1L << 24) - 1;
+
 // Checks a cache's shape and fills the map (page_table null: contiguous); what: the entry's name.
 inline int q8_map(Q8Map* m, const char* what, const int* page_table, bool paged, int max_pages,
                   int page_size, int n_pages, int Hkv, int Dh, int capacity) {

@@ -95,6 +95,22 @@ def test_shapes(name, args):
         assert rc(name, args, bf16=2) == INVALID
 
 
+@pytest.mark.parametrize("name,args", ATTENTION + CACHE)
+@pytest.mark.parametrize("dh", [16, 64])
+def test_more_rows_than_a_grid_holds(name, args, dh):
+    """Sizes that are ints each, but 2^24 workgroups or more together."""
+    if "Tq" in args:
+        for tq, hkv in ((1 << 30, 8), (1 << 25, 1), (1, 1 << 25), (0x7fffffff, 0x7fffffff)):
+            if dh == 64 and hkv == 1 and tq == 1 << 25:
+                tq <<= 4  # blocks of 16 rows
+            assert rc(name, args, Tq=tq, Hkv=hkv, Dh=dh, **(
+                {"stride": hkv * dh} if "stride" in args else {})) == UNSUPPORTED
+            assert b"too many" in _lib.lib().orator_last_error()
+    elif "B" in args:
+        assert rc(name, args, B=65535, Hq=65534, Hkv=2, Dh=dh) == UNSUPPORTED
+        assert rc(name, args, B=1 << 15, Hq=1 << 9, Hkv=1, Dh=dh) == UNSUPPORTED
+
+
 def test_token_logprobs():
     for n in ("rows", "vocab"):
         assert rc("token_logprobs", LOGPROBS, **{n: 0}) == OK
