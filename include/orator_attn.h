@@ -288,7 +288,9 @@ int orator_kv_read_q8_paged(const int8_t* kq, const float* ks, const int8_t* vq,
                             const int* d_pos0, void* stream);
 /* orator_gqa_decode over the 8-bit cache: q [Hq, Dh] fp32 attends the *d_pos + 1 keys, clamped to
  * the capacity (*d_pos < 0: no key, zeros).  Any Hq that is a multiple of Hkv.  The products are
- * exact in the codes; q and the softmax weights keep fp32 accuracy. */
+ * exact in the codes; q and the softmax weights keep fp32 accuracy.  A q that is not finite makes its
+ * own head NaN, a scale that is not the heads that attend it; q and scales are taken to have
+ * magnitudes between 2^-100 and 2^100, or 0. */
 int orator_gqa_decode_q8(const float* q, const int8_t* kq, const float* ks, const int8_t* vq,
                          const float* vs, float* out, int Hq, int Hkv, int Dh, const int* d_pos,
                          int capacity, float scale, void* stream);
@@ -308,7 +310,9 @@ int orator_gqa_decode_q8_paged(const float* q, const int8_t* kq, const float* ks
  * shared_len, none (zeros) where d_pos[b] < 0.  Keys of unmapped pages (negative or >= n_pages)
  * are not attended.  shared_len in [0, max_pages * page_size], page_size a power of two >= 16, any
  * B, any Hq that is a multiple of Hkv; Dh a multiple of 16, at most 256 (64 and 128 run on the
- * matrix cores).  Results as orator_gqa_decode_paged's, to fp32 rounding. */
+ * matrix cores).  Results as orator_gqa_decode_paged's, to fp32 rounding, for finite q and keys and
+ * values of magnitudes between 2^-100 and 2^100, or 0; a q, or an attended key or value, that is not
+ * finite may make what it enters NaN (an infinite score too). */
 int orator_gqa_decode_shared_paged(const float* q, const uint16_t* kpool, const uint16_t* vpool,
                                    const int* page_table, int max_pages, int page_size,
                                    int n_pages, const int* d_pos, int shared_len, float* out,
