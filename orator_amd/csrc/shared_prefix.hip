@@ -43,6 +43,8 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTile = 32;     // keys per wave tile
 constexpr int kCols = 32;     // query columns of a unit
+constexpr int kOwnHeads = 8;  // heads of an own unit: 4 columns each
+constexpr int kMaxOwn = 128;  // own units per stream, at most: a wave of the second kernel joins them
 constexpr float kSlack = 8.0f;
 // instruction kinds of __builtin_amdgcn_sched_group_barrier
 constexpr int kMfma = 0x008, kDsRead = 0x100;
@@ -55,7 +57,7 @@ struct SharedArgs {
   int col_blocks;   // blocks of 32 rows of the batch
   int n_pre;        // prefix units per (kv head, column block)
   int pre_tiles;    // tiles per prefix unit
-  int n_own;        // own units per (stream, kv head, chunk of 32 heads)
+  int n_own;        // own units (waves) per (stream, kv head, chunk of kOwnHeads heads)
   int own_chunks;
   int slots;        // n_pre + n_own: partials per (stream, head)
   float* part_o;    // [B * Hq][slots][Dh]
@@ -110,17 +112,37 @@ struct Tile {
   bool mapped0, mapped1;  // the tile's two blocks
 };
 
+// The page-table entries of a wave's tiles, 32 tiles at a time: lane 2 j + i holds the entry of block i
+// of tile first + j * stride.  The next tile's place is at hand whenever its loads can go out (looked up
+// per tile, the wave waited for the table each time: 64 streams of 1 to 512 keys 36 us instead of 27).
+struct TilePages {
+  int entry;
+  int at = 0;  // j of the next tile
+
+  __device__ __forceinline__ void fetch(const Q8Map& m, int row_b, int first, int stride, int lane) {
+    const long blk = 2 * (first + static_cast<long>(lane >> 1) * stride) + (lane & 1);
+    entry = m.page(row_b, static_cast<int>(min(blk, static_cast<long>(m.capacity / kQ8Block - 1))));
+    at = 0;
+  }
+  // Pages of tile `tile`, which follows the one asked for last; -1: unmapped.
+  __device__ __forceinline__ void next(const Q8Map& m, int row_b, int tile, int stride, int lane, int* p0,
+                                       int* p1) {
+    if (at == 32) fetch(m, row_b, tile, stride, lane);
+    *p0 = __builtin_amdgcn_readlane(entry, 2 * at);
+    *p1 = __builtin_amdgcn_readlane(entry, 2 * at + 1);
+    ++at;
+  }
+};
+
 // The rows of a bf16 tile in the pool.
 struct TileRows {
   long r0, r1;            // of its two blocks' first keys
   bool mapped0, mapped1;  // (unmapped: rows of page 0, which are masked)
 };
-__device__ __forceinline__ TileRows tile_rows(const SharedArgs& a, int row_b, int tile, int last_blk) {
-  const int b0 = min(2 * tile, last_blk), b1 = min(2 * tile + 1, last_blk);
-  const int p0 = a.map.page(row_b, b0), p1 = a.map.page(row_b, b1);
-  const int bs = a.map.block_shift, msk = (1 << bs) - 1;
-  return {((static_cast<long>(max(p0, 0)) << bs) + (b0 & msk)) << 4,
-          ((static_cast<long>(max(p1, 0)) << bs) + (b1 & msk)) << 4, p0 >= 0, p1 >= 0};
+__device__ __forceinline__ TileRows tile_rows(const Q8Map& m, int p0, int p1, int tile) {
+  const int bs = m.block_shift, msk = (1 << bs) - 1;
+  return {((static_cast<long>(max(p0, 0)) << bs) + (2 * tile & msk)) << 4,
+          ((static_cast<long>(max(p1, 0)) << bs) + ((2 * tile + 1) & msk)) << 4, p0 >= 0, p1 >= 0};
 }
 // A bf16 tile of K or V, rows as they lie, whole lines: DH / 8 lanes per row, rows in order.
 template <int DH>
@@ -143,19 +165,19 @@ __device__ __forceinline__ int dim_of(int s, int h) {
   return Q8 ? 32 * (s >> 1) + 16 * h + 8 * (s & 1) : 16 * s + 8 * h;
 }
 
-// An 8-bit tile.
+// An 8-bit tile of pages p0 and p1.
 template <int DH>
-__device__ __forceinline__ void load_tile(Tile<true, DH>& t, const SharedArgs& a, int row_b, int kvh,
-                                          int tile, int last_blk, int lane) {
-  const int b0 = min(2 * tile, last_blk), b1 = min(2 * tile + 1, last_blk);
+__device__ __forceinline__ void load_tile(Tile<true, DH>& t, const SharedArgs& a, int p0, int p1, int kvh,
+                                          int tile, int lane) {
   const int h = lane >> 5;
   const bool second = lane & 4;                       // K: the block of tile row lane & 31
   const int at = 4 * ((lane >> 3) & 3) + (lane & 3);  // and its place there
-  long n0 = a.map.block(row_b, b0, kvh), n1 = a.map.block(row_b, b1, kvh);
-  t.mapped0 = n0 >= 0;
-  t.mapped1 = n1 >= 0;
-  n0 = max(n0, 0L);  // unmapped: block 0 is read, its keys are masked
-  n1 = max(n1, 0L);
+  t.mapped0 = p0 >= 0;
+  t.mapped1 = p1 >= 0;
+  // unmapped: a block of page 0 is read, its keys are masked
+  const int bs = a.map.block_shift, msk = (1 << bs) - 1;
+  const long n0 = ((static_cast<long>(max(p0, 0)) * a.p.Hkv + kvh) << bs) + (2 * tile & msk);
+  const long n1 = ((static_cast<long>(max(p1, 0)) * a.p.Hkv + kvh) << bs) + ((2 * tile + 1) & msk);
   const int8_t* k = a.p.kq + ((second ? n1 : n0) * kQ8Block + at) * DH + 16 * h;
   const long nv = h ? n1 : n0;
   const int8_t* v = a.p.vq + (nv * DH + (lane & 31)) * kQ8Block;
@@ -177,116 +199,67 @@ constexpr int kKStride = DH + 8;   // of a K row
 template <int DH>
 constexpr int kQStride = DH + 8;   // and of a q row
 
-template <bool Q8, int DH>
-__global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs a) {
+// A wave's softmax state and sums: of query column lane & 31, dims 32 n + 8 (r >> 2) + 4 (lane >> 5) +
+// (r & 3) in o[n][r]; l is this lane's share.
+template <int DH>
+struct ColState {
+  float m = -INFINITY, l = 0.0f;
+  f32x16_t o[DH / 32] = {};
+};
+
+// A wave's tiles `tile`, tile + stride, ... of keys [lo, hi) through table row row_b; pages: theirs.
+// prepare() runs once the first tile's loads are on the way, and makes q ready for `q`: with OWN k-step
+// s's operand is q.at(s), one term a column, else q.at(s, term).  vt: the wave's buffer for a bf16 tile
+// in LDS.
+template <bool Q8, int DH, bool OWN, typename Query, typename Prepare>
+__device__ __forceinline__ void attend_tiles(ColState<DH>& st, const SharedArgs& a, int row_b, int kvh,
+                                             int lo, int hi, int tile, int stride, TilePages& pages,
+                                             uint16_t* vt, int lane, const Query& q, Prepare&& prepare) {
   constexpr int NS = DH / 16;  // k-steps of the first product
   constexpr int ND = DH / 32;  // dim blocks of the second
-  constexpr int OS = DH + 4;   // floats of an output row in LDS
-  constexpr size_t kQTerm = kCols * kQStride<DH>;  // elements of a term of q
-  constexpr size_t kQBytes = 3 * kQTerm * 2;
-  constexpr size_t kVBytes = Q8 ? 0 : kTile * kVStride<DH> * 2;
-  constexpr size_t kOBytes = kCols * OS * 4;
-  // q's terms and the waves' V tiles; then the waves' outputs
-  constexpr size_t kWork = kQBytes + kWaves * kVBytes;
-  __shared__ __align__(16) unsigned char smem[kWork > kWaves * kOBytes ? kWork : kWaves * kOBytes];
-  __shared__ float s_m[kWaves][kCols], s_l[kWaves][kCols];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = lane >> 5, col = lane & 31;
-  const int G = a.G, Hq = a.p.Hq, Hkv = a.p.Hkv, P = a.p.shared_len;
-
-  // ---- the unit: its columns, table row and keys [lo, hi) ----
-  const int kvh = blockIdx.x % Hkv;
-  int u = blockIdx.x / Hkv;
-  // the prefix's units first: they are the longer ones
-  const int n_prefix = a.col_blocks * a.n_pre;
-  const bool prefix = u < n_prefix;
-  if (!prefix) u -= n_prefix;
-  int row_b, lo, hi, slot, first_row;  // first_row: of the batch's rows b G + g (prefix), the head (own)
-  if (prefix) {
-    const int part = u / a.col_blocks;
-    first_row = (u % a.col_blocks) * kCols;
-    row_b = 0;
-    // (in 64 bits: the last range's end may pass 2^31)
-    const long from = static_cast<long>(part) * a.pre_tiles * kTile;
-    lo = static_cast<int>(min(from, static_cast<long>(P)));
-    hi = static_cast<int>(min(from + static_cast<long>(a.pre_tiles) * kTile, static_cast<long>(P)));
-    slot = part;
-  } else {
-    const int part = u % a.n_own;
-    u /= a.n_own;
-    first_row = (u % a.own_chunks) * kCols;
-    const int b = u / a.own_chunks;
-    const int S = stream_len(a, b);
-    const int first = S < P ? 0 : P;
-    row_b = S < P ? 0 : b;
-    u = b;
-    // whole tiles, counted from the tile that `first` lies in (key numbers past 2^31 in 64 bits)
-    const int t0 = first / kTile, n = (S + kTile - 1) / kTile - t0;
-    const long per = (n + a.n_own - 1) / a.n_own;
-    lo = static_cast<int>(max(static_cast<long>(first), min((t0 + part * per) * kTile, static_cast<long>(S))));
-    hi = static_cast<int>(min((t0 + (part + 1) * per) * kTile, static_cast<long>(S)));
-    slot = a.n_pre + part;
-  }
-  // stream and head (of the kv head's G) of column c; false: there is none
-  auto column = [&](int c, int* b, int* g) {
-    if (prefix) {
-      *b = (first_row + c) / G;
-      *g = (first_row + c) % G;
-      return *b < a.p.B;
-    }
-    *b = u;
-    *g = first_row + c;
-    return *g < G;
-  };
-
-  float m = -INFINITY, l = 0.0f;
-  f32x16_t o[ND] = {};
+  constexpr int NT = OWN ? 1 : 3;  // products of an operand pair
+  const int h = lane >> 5;
   const int t_end = hi > lo ? (hi + kTile - 1) / kTile : 0;
-  int tile = lo / kTile + wave;
-  const int last_blk = (hi - 1) >> 4;
   Tile<Q8, DH> nxt;
-  const long rs = static_cast<long>(Hkv) * DH;
+  const long rs = static_cast<long>(a.p.Hkv) * DH;
   TileRows rows{};  // bf16: of the tile in nxt
+  auto load_codes = [&](auto& t, int at) {
+    int p0, p1;
+    pages.next(a.map, row_b, at, stride, lane, &p0, &p1);
+    load_tile(t, a, p0, p1, kvh, at, lane);
+  };
+  auto find_rows = [&](int at) {
+    int p0, p1;
+    pages.next(a.map, row_b, at, stride, lane, &p0, &p1);
+    return tile_rows(a.map, p0, p1, at);
+  };
   if (tile < t_end) {
     if constexpr (Q8) {
-      load_tile(nxt, a, row_b, kvh, tile, last_blk, lane);
+      load_codes(nxt, tile);
     } else {
-      rows = tile_rows(a, row_b, tile, last_blk);
+      rows = find_rows(tile);
       load_rows<DH>(nxt.k, a.p.kpool, rows, rs, kvh, lane);
       load_rows<DH>(nxt.v, a.p.vpool, rows, rs, kvh, lane);
     }
   }
-
-  // ---- q as three terms in LDS, rows of columns; columns that there are not hold zeros ----
-  uint16_t* qt = reinterpret_cast<uint16_t*>(smem);
-  if (t_end > 0) {
-    for (int i = tid; i < kCols * (DH / 8); i += 64 * kWaves) {
-      const int c = i / (DH / 8), d = 8 * (i % (DH / 8));
-      int b, g;
-      float x[8] = {};
-      if (column(c, &b, &g)) {
-        const float* row = a.p.q + (static_cast<long>(b) * Hq + kvh * G + g) * DH + d;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = row[e] * a.scale_log2e;
-      }
-      uint4 t[3];
-      split3(x, t);
-#pragma unroll
-      for (int k = 0; k < 3; ++k)
-        *reinterpret_cast<uint4*>(qt + k * kQTerm + c * kQStride<DH> + d) = t[k];
-    }
-  }
-  lds_barrier();  // the first tile's loads stay on the way
-  const uint16_t* qcol = qt + col * kQStride<DH>;
-  uint16_t* vt = reinterpret_cast<uint16_t*>(smem + kQBytes + wave * kVBytes);
+  prepare(tile < t_end);
+  // OWN: which of w's terms this lane's column holds: w less its first (1), and less its second (2)
+  const uint32_t drop1 = OWN && (lane & 3) >= 1 ? 0xffff0000u : 0u;
+  const uint32_t drop2 = OWN && (lane & 3) >= 2 ? 0xffff0000u : 0u;
 
   auto work = [&](Tile<Q8, DH>& cur) __attribute__((always_inline)) {
     const int key0 = kTile * tile + 16 * h;  // this lane's 16 keys
     const bool mapped0 = Q8 ? cur.mapped0 : rows.mapped0, mapped1 = Q8 ? cur.mapped1 : rows.mapped1;
-    const bool mapped = h ? mapped1 : mapped0;
+    // Keeps y of the lane's keys that are attended, puts `none` for the others; one compare each, no
+    // branches.
+    auto mask = [&](float (&y)[16], float none) {
+      const int first = max(lo - key0, 0);
+      const uint32_t n = (h ? mapped1 : mapped0) ? static_cast<uint32_t>(max(hi - key0 - first, 0)) : 0u;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = static_cast<uint32_t>(i - first) < n ? y[i] : none;
+    };
     const bool whole = mapped0 && mapped1 && kTile * tile >= lo && kTile * (tile + 1) <= hi;
-    const bool more = tile + kWaves < t_end;  // bf16: the next tile takes this one's registers
+    const bool more = tile + stride < t_end;  // bf16: the next tile takes this one's registers
     constexpr int LPR = DH / 8, RPI = 64 / LPR;
     if constexpr (!Q8) {
 #pragma unroll
@@ -298,12 +271,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
 #pragma unroll
         for (int i = 0; i < DH / 16; ++i) {
           const int key = kTile * tile + RPI * i + lane / LPR;
-          if (!(RPI * i < 16 ? mapped0 : mapped1) || key < lo || key >= hi)
-            cur.v[i] = u32x4_t{0, 0, 0, 0};
+          const bool in = (RPI * i < 16 ? mapped0 : mapped1) & (key >= lo) & (key < hi);
+          cur.v[i] &= in ? ~0u : 0u;
         }
       }
       if (more) {
-        rows = tile_rows(a, row_b, tile + kWaves, last_blk);
+        rows = find_rows(tile + stride);
         load_rows<DH>(cur.k, a.p.kpool, rows, rs, kvh, lane);
       }
       wave_lds_sync();
@@ -324,20 +297,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
         kf = *reinterpret_cast<const uint4*>(krow + 16 * s);
       }
 #pragma unroll
-      for (int k = 2; k >= 0; --k) {
-        const uint4 qf = *reinterpret_cast<const uint4*>(qcol + k * kQTerm + dim_of<Q8>(s, h));
-        sc = mfma32(as_bf16x8(kf), as_bf16x8(qf), sc);
-      }
+      for (int k = NT - 1; k >= 0; --k) sc = mfma32(as_bf16x8(kf), as_bf16x8(q.at(s, k)), sc);
     }
     if constexpr (!Q8) {
-      // a k-step's operands are read ahead of the products of the one before
-      __builtin_amdgcn_sched_group_barrier(kDsRead, 8, 0);
+      if constexpr (!OWN) {
+        // a k-step's operands are read ahead of the products of the one before
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 8, 0);
 #pragma unroll
-      for (int s = 0; s < NS - 2; ++s) {
-        __builtin_amdgcn_sched_group_barrier(kMfma, 3, 0);
-        __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+        for (int s = 0; s < NS - 2; ++s) {
+          __builtin_amdgcn_sched_group_barrier(kMfma, 3, 0);
+          __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, 6, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(kMfma, 6, 0);
       // V takes K's place
       wave_lds_sync();
 #pragma unroll
@@ -350,47 +322,50 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       x[i] = sc[i];
+      if constexpr (OWN) x[i] = quad_sum(x[i]);  // a head's terms are its quad's columns
       if constexpr (Q8) x[i] *= reinterpret_cast<const float*>(cur.ks)[i];
     }
-    if (!whole) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (!mapped || key0 + i < lo || key0 + i >= hi) x[i] = -INFINITY;
-    }
+    if (!whole) mask(x, -INFINITY);
     float mx = x[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
     mx = xor32_max(mx);
-    if (__any(mx > m + kSlack)) {  // m is -infinity before the first key
-      const float mn = fmaxf(m, mx);
+    if (__any(mx > st.m + kSlack)) {  // m is -infinity before the first key
+      const float mn = fmaxf(st.m, mx);
       const float ref = mn == -INFINITY ? 0.0f : mn;
-      const float c = fast_exp2(m - ref);
-      l *= c;
+      const float c = fast_exp2(st.m - ref);
+      st.l *= c;
 #pragma unroll
       for (int n = 0; n < ND; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[n][i] *= c;
-      m = mn;
+        for (int i = 0; i < 16; ++i) st.o[n][i] *= c;
+      st.m = mn;
     }
-    const float ref = m == -INFINITY ? 0.0f : m;
+    const float ref = st.m == -INFINITY ? 0.0f : st.m;
     float w[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       w[i] = fast_exp2(x[i] - ref);
-      l += w[i];
+      st.l += w[i];
       if constexpr (Q8) w[i] *= reinterpret_cast<const float*>(cur.vs)[i];
     }
-    if (Q8 && !whole) {  // a scale behind the last key may be anything
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (!mapped || key0 + i < lo || key0 + i >= hi) w[i] = 0.0f;
-    }
-    uint4 wt[2][3];
+    if (Q8 && !whole) mask(w, 0.0f);  // a scale behind the last key may be anything
+    uint4 wt[2][NT];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const float y[8] = {w[8 * s],     w[8 * s + 1], w[8 * s + 2], w[8 * s + 3],
-                          w[8 * s + 4], w[8 * s + 5], w[8 * s + 6], w[8 * s + 7]};
-      split3(y, wt[s]);
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = w[8 * s + i];
+        if constexpr (OWN) {
+          y[i] -= __uint_as_float(__float_as_uint(y[i]) & drop1);
+          y[i] -= __uint_as_float(__float_as_uint(y[i]) & drop2);
+        }
+      }
+      if constexpr (OWN)
+        wt[s][0] = make_uint4(upper2(y[0], y[1]), upper2(y[2], y[3]), upper2(y[4], y[5]), upper2(y[6], y[7]));
+      else
+        split3(y, wt[s]);
     }
     if constexpr (!Q8) wave_lds_sync();
 #pragma unroll
@@ -410,7 +385,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
           vf = make_uint4(x0.x, x0.y, x1.x, x1.y);
         }
 #pragma unroll
-        for (int k = 2; k >= 0; --k) o[n] = mfma32(as_bf16x8(vf), as_bf16x8(wt[s][k]), o[n]);
+        for (int k = NT - 1; k >= 0; --k) st.o[n] = mfma32(as_bf16x8(vf), as_bf16x8(wt[s][k]), st.o[n]);
       }
     }
     if constexpr (!Q8) wave_lds_sync();  // the tile's buffer is written again
@@ -419,34 +394,213 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
     // two tiles' registers in turn: the next one is loaded while one is worked on
     Tile<Q8, DH> other;
     while (tile < t_end) {
-      if (tile + kWaves < t_end) load_tile(other, a, row_b, kvh, tile + kWaves, last_blk, lane);
+      if (tile + stride < t_end) load_codes(other, tile + stride);
       work(nxt);
-      tile += kWaves;
+      tile += stride;
       if (tile >= t_end) break;
-      if (tile + kWaves < t_end) load_tile(nxt, a, row_b, kvh, tile + kWaves, last_blk, lane);
+      if (tile + stride < t_end) load_codes(nxt, tile + stride);
       work(other);
-      tile += kWaves;
+      tile += stride;
     }
   } else {
-    for (; tile < t_end; tile += kWaves) work(nxt);
+    for (; tile < t_end; tile += stride) work(nxt);
   }
+  st.l = xor32_sum(st.l);
+}
+
+// q of an own unit: column 4 g + t holds term t of head g (t = 3: zeros).  Held in registers; beside
+// two tiles of the 8-bit cache there is no room, each lane keeps its operands in LDS.
+template <bool Q8, int DH>
+struct OwnQuery {
+  uint4 f[Q8 ? 1 : DH / 16];
+  uint4* mine;  // Q8: this lane's, 64 apart
+
+  __device__ __forceinline__ uint4 at(int s, int) const {
+    if constexpr (Q8)
+      return mine[64 * s];
+    else
+      return f[s];
+  }
+  // row: the first head's q
+  __device__ __forceinline__ void load(const float* row, int heads, float scale, int lane) {
+    const int g = (lane & 31) >> 2, t = lane & 3, h = lane >> 5;
+    const uint32_t drop1 = t >= 1 ? 0xffff0000u : 0u, drop2 = t >= 2 ? 0xffff0000u : 0u;
+    const bool in = g < heads && t < 3;
+    const float* from = row + static_cast<long>(min(g, heads - 1)) * DH;
+    // all of it on its way before any is worked on, and no branch between
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    f4 raw[DH / 8];
+#pragma unroll
+    for (int i = 0; i < DH / 8; ++i)
+      raw[i] = *reinterpret_cast<const f4*>(from + dim_of<Q8>(i >> 1, h) + 4 * (i & 1));
+#pragma unroll
+    for (int s = 0; s < DH / 16; ++s) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = in ? raw[2 * s + (e >> 2)][e & 3] * scale : 0.0f;
+        x[e] -= __uint_as_float(__float_as_uint(x[e]) & drop1);
+        x[e] -= __uint_as_float(__float_as_uint(x[e]) & drop2);
+      }
+      const uint4 op = make_uint4(upper2(x[0], x[1]), upper2(x[2], x[3]), upper2(x[4], x[5]), upper2(x[6], x[7]));
+      if constexpr (Q8)
+        mine[64 * s] = op;
+      else
+        f[s] = op;
+    }
+  }
+};
+
+// An own unit: one wave, up to 8 heads of one stream, a range of its keys.
+template <bool Q8, int DH>
+__device__ __forceinline__ void own_unit(const SharedArgs& a, long unit, uint16_t* vt, uint4* lds_q,
+                                         int lane) {
+  // units beside each other are the heads of one range: what they read lies side by side
+  const int chunk = static_cast<int>(unit % a.own_chunks);
+  unit /= a.own_chunks;
+  const int kvh = static_cast<int>(unit % a.p.Hkv);
+  unit /= a.p.Hkv;
+  const int part = static_cast<int>(unit % a.n_own);
+  if (unit / a.n_own >= a.p.B) return;
+  const int b = static_cast<int>(unit / a.n_own);
+  // every n_own-th tile from the one that the prefix ends in: where the wave begins does not depend on
+  // the stream's length, which comes from memory with the pages
+  const int P = a.p.shared_len;
+  int first = P, row_b = b, tile = P / kTile + part;
+  TilePages pages;
+  pages.fetch(a.map, row_b, tile, a.n_own, lane);
+  const int S = stream_len(a, b);
+  if (S < P) {  // uniform
+    first = 0, row_b = 0, tile = part;
+    pages.fetch(a.map, row_b, tile, a.n_own, lane);
+  }
+  const int heads = min(a.G - chunk * kOwnHeads, kOwnHeads);
+  const long head0 = static_cast<long>(b) * a.p.Hq + kvh * a.G + chunk * kOwnHeads;
+  ColState<DH> st;
+  OwnQuery<Q8, DH> q;
+  q.mine = lds_q + lane;
+  attend_tiles<Q8, DH, true>(st, a, row_b, kvh, first, S, tile, a.n_own, pages, vt, lane, q, [&](bool any) {
+    if (any) q.load(a.p.q + head0 * DH, heads, a.scale_log2e, lane);
+  });
+  const int g = (lane & 31) >> 2, t = lane & 3, h = lane >> 5;
+  const long ps = (head0 + g) * a.slots + a.n_pre + part;
+#pragma unroll
+  for (int i = 0; i < DH / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = quad_sum(t == 3 ? 0.0f : st.o[i][4 * r + e]);
+      if (t == r && g < heads)
+        *reinterpret_cast<float4*>(a.part_o + ps * DH + 32 * i + 8 * r + 4 * h) =
+            make_float4(x[0], x[1], x[2], x[3]);
+    }
+  if (lane < 32 && t == 0 && g < heads) {
+    a.part_ml[2 * ps] = st.m;
+    a.part_ml[2 * ps + 1] = st.l;
+  }
+}
+
+// q of a prefix unit's columns as three terms in LDS.
+template <bool Q8, int DH>
+struct PrefixQuery {
+  static constexpr size_t kTerm = kCols * kQStride<DH>;  // elements of a term
+  const uint16_t* col;  // this lane's column
+  int h;
+  __device__ __forceinline__ uint4 at(int s, int k) const {
+    return *reinterpret_cast<const uint4*>(col + k * kTerm + dim_of<Q8>(s, h));
+  }
+};
+
+template <bool Q8, int DH>
+__global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs a) {
+  constexpr int ND = DH / 32;
+  constexpr int OS = DH + 4;   // floats of an output row in LDS
+  constexpr size_t kQTerm = PrefixQuery<Q8, DH>::kTerm;
+  constexpr size_t kQBytes = 3 * kQTerm * 2;
+  constexpr size_t kVBytes = Q8 ? 0 : kTile * kVStride<DH> * 2;
+  constexpr size_t kOBytes = kCols * OS * 4;
+  // q's terms and the waves' bf16 tiles; then the waves' outputs
+  constexpr size_t kWork = kQBytes + kWaves * kVBytes;
+  __shared__ __align__(16) unsigned char smem[kWork > kWaves * kOBytes ? kWork : kWaves * kOBytes];
+  __shared__ float s_m[kWaves][kCols], s_l[kWaves][kCols];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, col = lane & 31;
+  const int G = a.G, Hq = a.p.Hq, Hkv = a.p.Hkv, P = a.p.shared_len;
+  uint16_t* vt = reinterpret_cast<uint16_t*>(smem + kQBytes + wave * kVBytes);
+
+  // ---- the unit: the prefix's first, they are the longer ones ----
+  const unsigned n_prefix = static_cast<unsigned>(a.col_blocks) * a.n_pre * Hkv;
+  if (blockIdx.x >= n_prefix) {
+    constexpr int kOps = 64 * (DH / 16);  // 16-byte operands of a wave's q
+    static_assert(!Q8 || kWaves * kOps * 16 <= sizeof(smem), "the waves' q take the outputs' place");
+    own_unit<Q8, DH>(a, static_cast<long>(blockIdx.x - n_prefix) * kWaves + wave, vt,
+                     reinterpret_cast<uint4*>(smem) + wave * kOps, lane);
+    return;
+  }
+  const int kvh = blockIdx.x % Hkv, u = blockIdx.x / Hkv;
+  const int part = u / a.col_blocks, first_row = (u % a.col_blocks) * kCols;
+  // (in 64 bits: the last range's end may pass 2^31)
+  const long from = static_cast<long>(part) * a.pre_tiles * kTile;
+  const int lo = static_cast<int>(min(from, static_cast<long>(P)));
+  const int hi = static_cast<int>(min(from + static_cast<long>(a.pre_tiles) * kTile, static_cast<long>(P)));
+  // stream and head (of the kv head's G) of column c; false: there is none
+  auto column = [&](int c, int* b, int* g) {
+    *b = (first_row + c) / G;
+    *g = (first_row + c) % G;
+    return *b < a.p.B;
+  };
+  ColState<DH> st;
+  uint16_t* qt = reinterpret_cast<uint16_t*>(smem);
+  const PrefixQuery<Q8, DH> q{qt + col * kQStride<DH>, h};
+  const int tile = lo / kTile + wave;
+  TilePages pages;
+  pages.fetch(a.map, 0, tile, kWaves, lane);
+  attend_tiles<Q8, DH, false>(st, a, 0, kvh, lo, hi, tile, kWaves, pages, vt, lane, q, [&](bool) {
+    // rows of columns; columns that there are not hold zeros.  Every load is on its way before the first
+    // is waited for
+    constexpr int N = kCols * (DH / 8) / (64 * kWaves);
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    f4 raw[N][2];
+    bool in[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = tid + j * 64 * kWaves;
+      int b, g;
+      in[j] = column(i / (DH / 8), &b, &g);
+      const float* row = a.p.q + (static_cast<long>(min(b, a.p.B - 1)) * Hq + kvh * G + g) * DH + 8 * (i % (DH / 8));
+      raw[j][0] = *reinterpret_cast<const f4*>(row);
+      raw[j][1] = *reinterpret_cast<const f4*>(row + 4);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = tid + j * 64 * kWaves, c = i / (DH / 8), d = 8 * (i % (DH / 8));
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = in[j] ? raw[j][e >> 2][e & 3] * a.scale_log2e : 0.0f;
+      uint4 t[3];
+      split3(x, t);
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        *reinterpret_cast<uint4*>(qt + k * kQTerm + c * kQStride<DH> + d) = t[k];
+    }
+    lds_barrier();  // the first tile's loads stay on the way
+  });
 
   // ---- the waves joined in LDS ----
   __syncthreads();
   float* so = reinterpret_cast<float*>(smem + wave * kOBytes);
-  l = xor32_sum(l);
   if (h == 0) {
-    s_m[wave][col] = m;
-    s_l[wave][col] = l;
+    s_m[wave][col] = st.m;
+    s_l[wave][col] = st.l;
   }
-  int unused_b, unused_g;
-  if (column(col, &unused_b, &unused_g))
 #pragma unroll
   for (int n = 0; n < ND; ++n)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       *reinterpret_cast<float4*>(so + col * OS + 32 * n + 8 * r + 4 * h) =
-          make_float4(o[n][4 * r], o[n][4 * r + 1], o[n][4 * r + 2], o[n][4 * r + 3]);
+          make_float4(st.o[n][4 * r], st.o[n][4 * r + 1], st.o[n][4 * r + 2], st.o[n][4 * r + 3]);
   __syncthreads();
   const float* all = reinterpret_cast<const float*>(smem);
   for (int i = tid; i < kCols * (DH / 4); i += 64 * kWaves) {
@@ -458,7 +612,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) M = fmaxf(M, s_m[w][c]);
     // a stream that is no column of the prefix leaves nothing there
-    const bool none = prefix && stream_len(a, b) < P;
+    const bool none = stream_len(a, b) < P;
     const float ref = M == -INFINITY ? 0.0f : M;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
@@ -470,7 +624,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
       r.z = fmaf(f, x.z, r.z);
       r.w = fmaf(f, x.w, r.w);
     }
-    const long ps = (static_cast<long>(b) * Hq + kvh * G + g) * a.slots + slot;
+    const long ps = (static_cast<long>(b) * Hq + kvh * G + g) * a.slots + part;
     if (none) {
       M = -INFINITY;
       L = 0.0f;
@@ -546,20 +700,21 @@ int launch_shared_prefix(const KeysProblem& p, const Q8Map& map, hipStream_t str
   a.G = p.Hq / p.Hkv;
   const long rows = static_cast<long>(p.B) * a.G;
   a.col_blocks = static_cast<int>((rows + kCols - 1) / kCols);
-  a.own_chunks = (a.G + kCols - 1) / kCols;
+  a.own_chunks = (a.G + kOwnHeads - 1) / kOwnHeads;
   const long cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  // Units of at least one tile per wave: up to one workgroup per CU for the prefix, and for the
-  // streams' own keys what is left of the two per CU that run at once.
+  // Prefix units of at least one tile per wave, up to one workgroup per CU; own units, a wave each, of
+  // at least a tile, as many as fill what is left of the two workgroups per CU that run at once.
   const long tiles = (p.shared_len + kTile - 1) / kTile;
   const long pre_units = static_cast<long>(a.col_blocks) * p.Hkv;
   long n_pre = tiles == 0 ? 0 : std::clamp(cus / pre_units, 1L, (tiles + kWaves - 1) / kWaves);
   a.pre_tiles = n_pre ? static_cast<int>((tiles + n_pre - 1) / n_pre) : 0;
   a.n_pre = a.pre_tiles ? static_cast<int>((tiles + a.pre_tiles - 1) / a.pre_tiles) : 0;
   const long own = (static_cast<long>(map.capacity) - p.shared_len + kTile - 1) / kTile + 1;
-  const long own_units = static_cast<long>(p.B) * p.Hkv * a.own_chunks;
-  a.n_own = static_cast<int>(std::clamp((2 * cus - pre_units * a.n_pre) / own_units, 1L, (own + kWaves - 1) / kWaves));
+  const long own_units = static_cast<long>(p.B) * a.own_chunks;
+  const long room = kWaves * (2 * cus - pre_units * a.n_pre);
+  a.n_own = static_cast<int>(std::clamp(room / (own_units * p.Hkv), 1L, std::min<long>(own, kMaxOwn)));
   a.slots = a.n_pre + a.n_own;
-  const long grid = pre_units * a.n_pre + own_units * a.n_own;
+  const long grid = pre_units * a.n_pre + (own_units * p.Hkv * a.n_own + kWaves - 1) / kWaves;
   if (grid > kMaxGroups256)
     return fail(ORATOR_ERR_UNSUPPORTED, "gqa_decode_shared: too many streams and heads");
   const size_t parts = static_cast<size_t>(p.B) * p.Hq * a.slots;
