@@ -1,20 +1,23 @@
 // Decode attention of a batch whose streams share a prefix, over the bf16 pool or the 8-bit cache:
 // the prefix's keys are read once for all streams, gfx950.
 //
-// For one kv head, the B G query rows of the batch against the prefix are a matrix product, and so
-// are a stream's G rows against its own keys (G of 32 columns used: its time is its memory's).
-// One kernel does both; a workgroup has one unit of work, 32 query columns and a range of keys:
-//  * prefix units: columns are rows (stream, head) b G + g of the batch, keys [0, P) through
-//    page-table row 0;
-//  * own units: columns are the G heads of one stream, keys [P, S_b) through its own row.  A stream
-//    with fewer keys than the prefix has none there and is no column of a prefix unit: its unit
-//    takes keys [0, S_b) of row 0.  So a unit's columns all attend the same keys, and a value that
-//    is not finite reaches no stream that does not attend it (0 * inf in a product is NaN).
+// For one kv head, the B G query rows of the batch against the prefix are a matrix product; a stream's
+// G rows against its own keys use few columns of one, and their time is their memory's.  One kernel
+// does both, in two kinds of units:
+//  * prefix units, a workgroup each: columns are 32 rows (stream, head) b G + g of the batch, keys a
+//    range of [0, P) through page-table row 0, which the waves take tile by tile in turn;
+//  * own units, a wave each: columns are up to 8 heads of one stream, keys every n_own-th tile of
+//    [P, S_b) through its own row.  A stream with fewer keys than the prefix has none there and is no
+//    column of a prefix unit: its units take keys [0, S_b) of row 0.  So a unit's columns all attend
+//    the same keys, and a value that is not finite reaches no stream that does not attend it (0 * inf
+//    in a product is NaN).
 //
 // Per 32-key tile of a wave, S^T = K Q^T and O^T += V^T W^T on mfma_f32_32x32x16_bf16:
 //  * q and the weights w enter as three bf16 terms (the top 8, middle 8 and last 8 bits of the
 //    fp32 significand, split by truncation: exact), K and V as they are (bf16, or int8 codes,
-//    which bf16 holds exactly): fp32 accuracy for 3 MFMAs per product.
+//    which bf16 holds exactly): fp32 accuracy for 3 MFMAs per product.  In an own unit a head's
+//    terms are the columns of a quad instead, and one MFMA does all: scores are the quad's sums, the
+//    outputs' terms are summed at the end.
 //  * a lane has one query column, and scores of 16 consecutive keys: tile row 8 a + 4 h + i is key
 //    16 h + 4 a + i, so lane half h holds block h of the tile and its registers are the B operand
 //    of the second product as they are.
@@ -22,15 +25,16 @@
 //    transposing read).  8-bit codes go from memory into the operands: K a half line of a row, V as
 //    it lies transposed.
 //  * softmax with a reference that follows the running maximum once it is 8 (log2) behind.
-// The waves of a workgroup take the range's tiles in turn and are joined in LDS; the units'
-// partials of a (stream, head) by a second kernel (joined by the last unit to finish, in the same
-// launch, the one that completes a block of columns joins 32 rows alone: B = 64, prefix 4096
-// measured 52 us instead of 41, B = 16 over the 8-bit cache 30 instead of 15).
+// A prefix unit's waves are joined in LDS; the units' partials of a (stream, head) by a second kernel
+// (joined by the last unit to finish, in the same launch, the one that completes a block of columns
+// joins 32 rows alone: B = 64, prefix 4096 measured 52 us instead of 41, B = 16 over the 8-bit cache 30
+// instead of 15).
 //
 // Measured, 16 q / 8 kv heads of 128, both launches: 64 streams behind 4096 keys with 1 to 512 of their
-// own, bf16, 37.9 us (85 MB: 16.5 us at a copy's rate); 16 behind 2048, 8-bit, 14.6 us; 6 behind 503,
-// bf16, 11.1 us.  A tile is 48 MFMAs (0.7 us) and some 430 VALU instructions; two waves per SIMD
-// overlap them to 1.3 us a tile, and a workgroup's start and end cost 7 us.
+// own, bf16, 28.4 us (85 MB: 16.5 us at a copy's rate; own keys by workgroups of four waves with three
+// MFMAs a product 37.9); 16 behind 2048, 8-bit, 15.1 us; 6 behind 503, bf16, 10.7 us.  A prefix tile is
+// 48 MFMAs (0.7 us) and some 430 VALU instructions, one wave after another 1.3 us per SIMD; the rest is
+// the chain page -> rows -> products -> partials -> join of two launches.
 #include <algorithm>
 #include <string>
 
@@ -113,8 +117,7 @@ struct Tile {
 };
 
 // The page-table entries of a wave's tiles, 32 tiles at a time: lane 2 j + i holds the entry of block i
-// of tile first + j * stride.  The next tile's place is at hand whenever its loads can go out (looked up
-// per tile, the wave waited for the table each time: 64 streams of 1 to 512 keys 36 us instead of 27).
+// of tile first + j * stride, so that a tile's loads go out without a look-up before them.
 struct TilePages {
   int entry;
   int at = 0;  // j of the next tile
@@ -144,8 +147,11 @@ __device__ __forceinline__ TileRows tile_rows(const Q8Map& m, int p0, int p1, in
   return {((static_cast<long>(max(p0, 0)) << bs) + (2 * tile & msk)) << 4,
           ((static_cast<long>(max(p1, 0)) << bs) + ((2 * tile + 1) & msk)) << 4, p0 >= 0, p1 >= 0};
 }
+// Rows that one unit reads (NT) are loaded past the caches' other lines: behind a kernel that left 256
+// MB of written lines there, 64 streams of 1 to 512 keys 20.8 us instead of 33.6 (of 8-bit codes, V
+// alone, whose lines a load covers: 28.6 instead of 30.2); no difference with clean caches.
 // A bf16 tile of K or V, rows as they lie, whole lines: DH / 8 lanes per row, rows in order.
-template <int DH>
+template <int DH, bool NT>
 __device__ __forceinline__ void load_rows(u32x4_t (&r)[DH / 16], const uint16_t* pool,
                                           const TileRows& t, long rs, int kvh, int lane) {
   constexpr int LPR = DH / 8, RPI = 64 / LPR;  // lanes per row, rows per load
@@ -154,7 +160,8 @@ __device__ __forceinline__ void load_rows(u32x4_t (&r)[DH / 16], const uint16_t*
   for (int i = 0; i < DH / 16; ++i) {
     const int row = RPI * i;  // a load's rows lie in one block (RPI divides 16): a uniform base
     const uint16_t* at = pool + ((row < 16 ? t.r0 : t.r1) + (row & 15)) * rs + kvh * DH;
-    r[i] = *reinterpret_cast<const u32x4_t*>(at + off);
+    const u32x4_t* from = reinterpret_cast<const u32x4_t*>(at + off);
+    r[i] = NT ? __builtin_nontemporal_load(from) : *from;
   }
 }
 
@@ -166,7 +173,7 @@ __device__ __forceinline__ int dim_of(int s, int h) {
 }
 
 // An 8-bit tile of pages p0 and p1.
-template <int DH>
+template <int DH, bool NT>
 __device__ __forceinline__ void load_tile(Tile<true, DH>& t, const SharedArgs& a, int p0, int p1, int kvh,
                                           int tile, int lane) {
   const int h = lane >> 5;
@@ -184,7 +191,10 @@ __device__ __forceinline__ void load_tile(Tile<true, DH>& t, const SharedArgs& a
 #pragma unroll
   for (int i = 0; i < DH / 32; ++i) t.k[i] = *reinterpret_cast<const u32x4_t*>(k + 32 * i);
 #pragma unroll
-  for (int i = 0; i < DH / 32; ++i) t.v[i] = *reinterpret_cast<const u32x4_t*>(v + 32 * i * kQ8Block);
+  for (int i = 0; i < DH / 32; ++i) {
+    const u32x4_t* from = reinterpret_cast<const u32x4_t*>(v + 32 * i * kQ8Block);
+    t.v[i] = NT ? __builtin_nontemporal_load(from) : *from;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     t.ks[i] = *reinterpret_cast<const float4*>(a.p.ks + nv * kQ8Block + 4 * i);
@@ -226,7 +236,7 @@ __device__ __forceinline__ void attend_tiles(ColState<DH>& st, const SharedArgs&
   auto load_codes = [&](auto& t, int at) {
     int p0, p1;
     pages.next(a.map, row_b, at, stride, lane, &p0, &p1);
-    load_tile(t, a, p0, p1, kvh, at, lane);
+    load_tile<DH, OWN>(t, a, p0, p1, kvh, at, lane);
   };
   auto find_rows = [&](int at) {
     int p0, p1;
@@ -238,8 +248,8 @@ __device__ __forceinline__ void attend_tiles(ColState<DH>& st, const SharedArgs&
       load_codes(nxt, tile);
     } else {
       rows = find_rows(tile);
-      load_rows<DH>(nxt.k, a.p.kpool, rows, rs, kvh, lane);
-      load_rows<DH>(nxt.v, a.p.vpool, rows, rs, kvh, lane);
+      load_rows<DH, OWN>(nxt.k, a.p.kpool, rows, rs, kvh, lane);
+      load_rows<DH, OWN>(nxt.v, a.p.vpool, rows, rs, kvh, lane);
     }
   }
   prepare(tile < t_end);
@@ -277,7 +287,7 @@ __device__ __forceinline__ void attend_tiles(ColState<DH>& st, const SharedArgs&
       }
       if (more) {
         rows = find_rows(tile + stride);
-        load_rows<DH>(cur.k, a.p.kpool, rows, rs, kvh, lane);
+        load_rows<DH, OWN>(cur.k, a.p.kpool, rows, rs, kvh, lane);
       }
       wave_lds_sync();
     }
@@ -316,7 +326,7 @@ __device__ __forceinline__ void attend_tiles(ColState<DH>& st, const SharedArgs&
       for (int i = 0; i < DH / 16; ++i)
         *reinterpret_cast<u32x4_t*>(vt + (RPI * i + lane / LPR) * kVStride<DH> + 8 * (lane % LPR)) =
             cur.v[i];
-      if (more) load_rows<DH>(cur.v, a.p.vpool, rows, rs, kvh, lane);
+      if (more) load_rows<DH, OWN>(cur.v, a.p.vpool, rows, rs, kvh, lane);
     }
     float x[16];
 #pragma unroll
@@ -442,7 +452,8 @@ struct OwnQuery {
         x[e] -= __uint_as_float(__float_as_uint(x[e]) & drop1);
         x[e] -= __uint_as_float(__float_as_uint(x[e]) & drop2);
       }
-      const uint4 op = make_uint4(upper2(x[0], x[1]), upper2(x[2], x[3]), upper2(x[4], x[5]), upper2(x[6], x[7]));
+      const uint4 op = make_uint4(upper2(x[0], x[1]), upper2(x[2], x[3]), upper2(x[4], x[5]),
+                                  upper2(x[6], x[7]));
       if constexpr (Q8)
         mine[64 * s] = op;
       else
@@ -569,7 +580,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(SharedArgs 
       const int i = tid + j * 64 * kWaves;
       int b, g;
       in[j] = column(i / (DH / 8), &b, &g);
-      const float* row = a.p.q + (static_cast<long>(min(b, a.p.B - 1)) * Hq + kvh * G + g) * DH + 8 * (i % (DH / 8));
+      const float* row = a.p.q + (static_cast<long>(min(b, a.p.B - 1)) * Hq + kvh * G + g) * DH +
+                         8 * (i % (DH / 8));
       raw[j][0] = *reinterpret_cast<const f4*>(row);
       raw[j][1] = *reinterpret_cast<const f4*>(row + 4);
     }
