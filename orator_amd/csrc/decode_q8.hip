@@ -16,8 +16,8 @@
 //    operand.  B = the V codes, [dim][16 keys] per block: the lane's 16 bytes as they lie in
 //    memory.  The four digit rows of a head come out in one lane, which adds them to its fp32 sums.
 //    Key (t, i) of a step's tile t is 16 g + 4 t + i for lane group g, so that A and B agree.
-//  So one 64-key step of one wave is 8 + 8 MFMAs of 16 cycles per 4 heads (Dh 128) and about 270
-//  VALU instructions, against 16.5 KB from HBM.
+//  So one 64-key step of one wave is 8 + 8 MFMAs of 16 cycles per 4 heads (Dh 128) and some 490 VALU
+//  instructions (counted over whole calls, with each wave's start and end), against 16.5 KB from HBM.
 //  * one workgroup = (a range of one stream's keys, kv head), 4 waves that take 64-key steps in
 //    turn; the next step's codes are loaded while the current one is worked on.  The streams share
 //    the workgroups of a kv head by their lengths, which every workgroup reads at entry (two
