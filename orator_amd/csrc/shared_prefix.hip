@@ -32,7 +32,8 @@
 //
 // Measured, 16 q / 8 kv heads of 128, both launches: 64 streams behind 4096 keys with 1 to 512 of their
 // own, bf16, 28.4 us (85 MB: 16.5 us at a copy's rate; own keys by workgroups of four waves with three
-// MFMAs a product 37.9); 16 behind 2048, 8-bit, 15.1 us; 6 behind 503, bf16, 10.7 us.  A prefix tile is
+// MFMAs a product 37.9; with written lines in the caches, 256 streams of up to 128 keys behind 1024 42
+// us instead of 56, 16 streams of 32 q heads on 2 kv heads 20.8 instead of 19.9); 16 behind 2048, 8-bit, 15.1 us; 6 behind 503, bf16, 10.7 us.  A prefix tile is
 // 48 MFMAs (0.7 us) and some 430 VALU instructions, one wave after another 1.3 us per SIMD; the rest is
 // the chain page -> rows -> products -> partials -> join of two launches.
 #include <algorithm>
